@@ -273,6 +273,35 @@ int pkcu_joint_add_act(const float *enc, const float *pred, float *out, int B, i
 int pkcu_argmax_rows(const float *logits, int32_t *out, long long n_rows, int V,
                      pkcu_stream_t stream);
 
+/* ── 8-bit activations ───────────────────────────────────────────────────────
+ * Rows in 8 bits with one fp32 scale each: what row m, column k holds stands
+ * for scales[m] * q[m, k]. No counterpart in the reference (its int8 weights
+ * meet fp32 activations). Element types: PKCU_DTYPE_F32 and PKCU_DTYPE_I8
+ * (section 4 below) and */
+#define PKCU_DTYPE_BF16 3
+#define PKCU_DTYPE_F16  4
+#define PKCU_DTYPE_E4M3 5   /* 8-bit float: 4 exponent and 3 mantissa bits, largest value 448 */
+
+/* Residual, root-mean-square norm and its 8-bit output in one pass over rows
+ * of D (x, y, x_out packed [n_rows, D] of type dtype: F32, BF16 or F16; gamma,
+ * bias [D] and scales [n_rows] fp32):
+ *   x_out  = x + alpha * (y + bias), rounded to dtype
+ *   n      = x_out * gamma / sqrt(mean(x_out^2) + eps)
+ *   scales = max|n| / Q per row, Q = 127 (qtype I8) or 448 (E4M3)
+ *   q      = n / scales rounded to nearest even, [n_rows, ldq] bytes (columns
+ *            from D on are left as they were)
+ * Arithmetic in fp32 (so entries up to about 1e18 in magnitude). x_out may be
+ * x. y NULL: no residual (bias must be NULL too), the norm is of x, and x_out
+ * may be NULL. bias may be NULL. A row of zeros gives q = 0 and scale 0; a row
+ * with a NaN or an infinity gives q = 0 and scale NaN. ldq a multiple of 16
+ * and q 16-byte aligned make the rows an operand of pkcu_wmatmul_q8. Pointers
+ * aligned to their type; 16-byte alignment (and D a multiple of 4, of 8 in 16
+ * bits) is the fast case. */
+int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, float alpha,
+                              const float *gamma, float eps, int dtype, void *x_out, void *q,
+                              int qtype, long long ldq, float *scales, int n_rows, int D,
+                              pkcu_stream_t stream);
+
 /* ── 3. sequence driver ──────────────────────────────────────────────────── */
 
 /* Non-GEMM parameters of one conformer block (csrc/parakeet.h:78-125). */

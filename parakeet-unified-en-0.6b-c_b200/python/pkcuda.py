@@ -20,6 +20,8 @@ D, H, DH, FF = 1024, 8, 128, 4096
 PKCU_CHANNEL_FIRST, PKCU_TIME_FIRST = 0, 1
 PKCU_GROUP_ALONG_K, PKCU_GROUP_ALONG_N = 0, 1
 PKCU_ACT_RELU, PKCU_ACT_TANH = 0, 1
+PKCU_DTYPE_F32, PKCU_DTYPE_I8, PKCU_DTYPE_I4 = 0, 1, 2
+PKCU_DTYPE_BF16, PKCU_DTYPE_F16, PKCU_DTYPE_E4M3 = 3, 4, 5
 PKCU_CHUNK_AUTO, PKCU_CHUNK_OFF, PKCU_CHUNK_ON = 0, 1, 2
 PKCU_OK, PKCU_ERR_ARG, PKCU_ERR_CUDA, PKCU_ERR_NOMEM = 0, 1, 2, 3
 PKCU_CHUNK_SIZE, PKCU_CHUNK_OVERLAP, PKCU_CHUNK_THRESHOLD = 400, 8, 500
@@ -64,7 +66,7 @@ EXPORTED = (
     "pkcu_weight_create", "pkcu_weight_destroy", "pkcu_wmatmul_work_bytes", "pkcu_wmatmul",
     "pkcu_wmatmul_bias_swish", "pkcu_wmatmul_bias_residual", "pkcu_wmatmul_qkv",
     "pkcu_encoder_nongemm_fused", "pkcu_conv_weight_create", "pkcu_pointwise_conv1d",
-    "pkcu_pointwise_conv1d_glu",
+    "pkcu_pointwise_conv1d_glu", "pkcu_residual_rms_norm_q8",
 )
 
 
@@ -200,6 +202,7 @@ _SIGS = {
     "pkcu_conv_weight_create": (I, [VP, I, I, I, VP, C.POINTER(VP)]),
     "pkcu_pointwise_conv1d": (I, [VP, VP, VP, VP, I, VP, VP]),
     "pkcu_pointwise_conv1d_glu": (I, [VP, VP, VP, VP, I, VP, VP]),
+    "pkcu_residual_rms_norm_q8": (I, [VP, VP, VP, F, VP, F, I, VP, VP, I, LL, VP, I, I, VP]),
 }
 
 _lib = None
@@ -259,6 +262,72 @@ def stream_handle(stream=None) -> int:
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+# ── 8-bit activations: tensors in, one call through the C ABI ─────────────────
+
+_TORCH_DTYPES = {}
+
+
+def dtype_of(t) -> int:
+    """PKCU_DTYPE_* of a torch tensor."""
+    if not _TORCH_DTYPES:
+        import torch
+        _TORCH_DTYPES.update({torch.float32: PKCU_DTYPE_F32, torch.bfloat16: PKCU_DTYPE_BF16,
+                              torch.float16: PKCU_DTYPE_F16, torch.int8: PKCU_DTYPE_I8,
+                              torch.float8_e4m3fn: PKCU_DTYPE_E4M3})
+    d = _TORCH_DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"no PKCU_DTYPE for {t.dtype}")
+    return d
+
+
+def _require(ok, what) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _vector(t, n, what):
+    """fp32 [n] on the GPU, packed (or None)."""
+    if t is not None:
+        import torch
+        _require(t.dtype == torch.float32 and t.is_cuda and t.is_contiguous() and t.numel() == n,
+                 f"{what}: a packed fp32 CUDA tensor of {n} entries is needed")
+
+
+def _call_on(t, stream, name, *args) -> None:
+    """call(name, *args, stream) on the device of t."""
+    import torch
+    if t.device.index != torch.cuda.current_device():
+        with torch.cuda.device(t.device):
+            call(name, *args, stream_handle(stream))
+    else:
+        call(name, *args, stream_handle(stream))
+
+
+def _same_device(t, *others) -> None:
+    for o in others:
+        _require(o is None or o.device == t.device, "tensors on different devices")
+
+
+def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream=None) -> None:
+    """pkcu_residual_rms_norm_q8 on tensors: x, y, x_out [n_rows, D]; q [n_rows,
+    >= D] int8 or float8_e4m3fn with packed columns; y, bias, x_out may be None
+    as in C."""
+    _require(x.dim() == 2 and x.is_cuda and x.is_contiguous(), "x: a packed [n_rows, D] CUDA tensor is needed")
+    rows, D = x.shape
+    for t, what in ((y, "y"), (x_out, "x_out")):
+        _require(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous()),
+                 f"{what}: the shape and type of x, packed, are needed")
+    _require(q.dim() == 2 and q.shape[0] == rows and q.shape[1] >= D and (q.stride(1) == 1 or q.shape[1] == 1),
+             "q: [n_rows, >= D] with packed columns is needed")
+    _vector(gamma, D, "gamma")
+    _vector(bias, D, "bias")
+    _vector(scales, rows, "scales")
+    _same_device(x, y, bias, gamma, x_out, q, scales)
+    _call_on(x, stream, "pkcu_residual_rms_norm_q8", x.data_ptr(), ptr(y), ptr(bias), alpha, gamma.data_ptr(),
+             eps, dtype_of(x), ptr(x_out), q.data_ptr(), dtype_of(q), q.stride(0) if rows > 1 else max(q.stride(0), D),
+             scales.data_ptr(), rows, D)
 
 
 class Seq:

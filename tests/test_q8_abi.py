@@ -1,0 +1,35 @@
+"""CPU: the 8-bit operators refuse bad arguments before any CUDA call."""
+import ctypes as C
+import os
+
+import pytest
+
+import pkcuda
+
+ERR_ARG = 1
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not os.path.exists(pkcuda.LIB_PATH):
+        pkcuda.build()
+    return pkcuda.lib()
+
+
+P = 4096   # stands for a device address: never read
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(n_rows=-1), "rows"), (dict(D=0), "rows"), (dict(D=(1 << 24) + 1), "rows"), (dict(dtype=1), "type"), (dict(dtype=5), "type"),
+    (dict(dtype=9), "type"), (dict(qtype=0), "output"), (dict(qtype=3), "output"), (dict(ldq=1023), "ldq"),
+    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"), (dict(x=None), "NULL"),
+    (dict(gamma=None), "NULL"), (dict(q=None), "NULL"), (dict(scales=None), "NULL"), (dict(x_out=None), "NULL"),
+    (dict(y=None), "bias"), (dict(x=P + 2), "aligned"), (dict(gamma=P + 1), "aligned"),
+    (dict(scales=P + 2), "aligned"), (dict(dtype=3, y=P + 1), "aligned")])
+def test_rms_norm_refusals(L, change, word):
+    a = dict(x=P, y=P, bias=P, alpha=1.0, gamma=P, eps=1e-5, dtype=0, x_out=P, q=P, qtype=1, ldq=1024, scales=P,
+             n_rows=4, D=1024)
+    a.update(change)
+    assert L.pkcu_residual_rms_norm_q8(*a.values(), None) == ERR_ARG
+    msg = L.pkcu_last_error().decode()
+    assert "pkcu_residual_rms_norm_q8" in msg and word in msg, msg
