@@ -35,31 +35,30 @@ struct RmsArgs {
 
 // ── what a row's statistics become ───────────────────────────────────────────
 
-struct RowQ {
-  float mul;    // t -> t mul pre is the value that is rounded
-  float pre;    // 2^100 for rows whose largest |t| is so small that Q / max|t| would overflow
-  float scale;
-};
+// q = round(t mul): what every thread of a row needs. mul 0: q is 0 (a row of
+// zeros, or one that stands for NaN).
 template <bool E4M3>
-__device__ __forceinline__ RowQ row_q(float ss, float amax, float eps, int D) {
-  constexpr float Q = E4M3 ? 448.0f : 127.0f;
-  RowQ o;
+struct Quant {
+  static constexpr float Q = E4M3 ? 448.0f : 127.0f;
+};
+__device__ __forceinline__ bool row_finite(float ss, float amax) { return ss < INFINITY && amax < INFINITY; }
+// Below this largest |t|, Q / max|t| would overflow; t is scaled up first.
+constexpr float kTiny = 0x1p-100f, kTinyUp = 0x1p100f;
+
+// The row's scale (one thread): a NaN or an infinity anywhere in the row (or
+// squares past fp32) makes it NaN, so that every entry stands for NaN.
+template <bool E4M3>
+__device__ __forceinline__ float row_scale(float ss, float amax, float eps, int D) {
+  if (!row_finite(ss, amax)) return __int_as_float(0x7fffffff);
+  if (amax == 0.0f) return 0.0f;
   const float r = 1.0f / sqrtf(ss / (float)D + eps);
-  o.pre = amax < 0x1p-100f ? 0x1p100f : 1.0f;
-  if (amax == 0.0f) {          // a row of zeros: q = 0, scale = 0
-    o.mul = 0.0f;
-    o.scale = 0.0f;
-  } else {
-    o.mul = Q / (amax * o.pre);
-    o.scale = amax * r / Q;
-  }
-  // a NaN or an infinity anywhere in the row (or squares past fp32): every
-  // entry stands for NaN, carried by the scale
-  if (!(ss < INFINITY) || !(amax < INFINITY)) {
-    o.mul = 0.0f;
-    o.scale = __int_as_float(0x7fffffff);
-  }
-  return o;
+  return amax * r / Quant<E4M3>::Q;
+}
+// Q / max|t|, 0 for a row whose q is 0; up: what t is multiplied by first.
+template <bool E4M3>
+__device__ __forceinline__ float row_mul(float ss, float amax, float &up) {
+  up = amax < kTiny ? kTinyUp : 1.0f;
+  return amax == 0.0f || !row_finite(ss, amax) ? 0.0f : Quant<E4M3>::Q / (amax * up);
 }
 
 // max that keeps a NaN
@@ -69,19 +68,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// t mul rounded to nearest even, as its 8-bit pattern; |t mul| <= Q (1 + 2^-22),
-// which rounds to Q at most, so nothing saturates. With mul = 0 (a row of
-// zeros, or one that stands for NaN) q is 0 whatever t is.
-template <bool E4M3>
-__device__ __forceinline__ unsigned char q8(float t, const RowQ &rq) {
-  if (rq.mul == 0.0f) return 0;
-  const float v = (t * rq.pre) * rq.mul;
-  if (E4M3) return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-  return (unsigned char)(signed char)__float2int_rn(v);
+// N entries t mul rounded to nearest even, as their 8-bit patterns, for finite
+// t; |t mul| <= Q (1 + 2^-22), which rounds to Q at most, so nothing saturates.
+// int8: t mul + 1.5 2^23 in one fused multiply-add rounds to an integer whose
+// two's complement is the sum's low byte.
+template <bool E4M3, int N>
+__device__ __forceinline__ void q8(const float *t, float mul, unsigned char *o) {
+  if constexpr (E4M3) {
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) {
+      const __nv_fp8x2_storage_t p = __nv_cvt_float2_to_fp8x2(make_float2(t[i] * mul, t[i + 1] * mul), __NV_SATFINITE, __NV_E4M3);
+      o[i] = (unsigned char)(p & 0xff);
+      o[i + 1] = (unsigned char)(p >> 8);
+    }
+    if (N & 1) o[N - 1] = __nv_cvt_float_to_fp8(t[N - 1] * mul, __NV_SATFINITE, __NV_E4M3);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) o[i] = (unsigned char)(__float_as_uint(fmaf(t[i], mul, 12582912.0f)) & 0xff);
+  }
 }
 
 // (ss, amax) over the TPR threads of a row. TPR 32: the row's warp, by
-// shuffles; else the whole CTA. red: 2 * 32 floats, used once per row.
+// shuffles; else the whole CTA. red: 64 floats, used once.
 template <int TPR>
 __device__ __forceinline__ void row_reduce(float &ss, float &amax, float *red) {
 #pragma unroll
@@ -130,18 +138,174 @@ __global__ void __launch_bounds__(256) rms_q8_long_kernel(RmsArgs a) {
     amax = max_nan(amax, fabsf(v * __ldg(a.gamma + i)));
   }
   row_reduce<256>(ss, amax, red);
-  const RowQ rq = row_q<E4M3>(ss, amax, a.eps, a.D);
+  float up;
+  const float mul = row_mul<E4M3>(ss, amax, up);
   unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
   const T *v = xo ? xo : x;   // each thread re-reads the entries that it wrote itself
-  for (int i = threadIdx.x; i < a.D; i += 256) q[i] = q8<E4M3>(to_f32(v[i]) * __ldg(a.gamma + i), rq);
-  if (threadIdx.x == 0) a.scales[row] = rq.scale;
+  for (int i = threadIdx.x; i < a.D; i += 256) {
+    const float t = to_f32(v[i]) * __ldg(a.gamma + i) * up;
+    unsigned char o = 0;
+    if (mul != 0.0f) q8<E4M3, 1>(&t, mul, &o);
+    q[i] = o;
+  }
+  if (threadIdx.x == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
+}
+
+// ── rows held in registers ────────────────────────────────────────────────────
+// TPR threads per row (a warp, eight rows to a CTA; or a whole CTA), each
+// holding EPT entries in chunks of VEC (16 bytes of the stream's type, or one
+// entry where rows are not 16-byte aligned), chunk c of the row at thread c mod
+// TPR, so every access of a warp is contiguous. All of a thread's loads of x
+// and y are issued before the first is used.
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T e[VEC];
+};
+
+template <typename T, int VEC, bool STREAM>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
+  Pack<T, VEC> r;
+  if constexpr (VEC == 1) {
+    r.e[0] = *p;
+  } else {
+    const float4 v = STREAM ? __ldcs(reinterpret_cast<const float4 *>(p)) : *reinterpret_cast<const float4 *>(p);
+    r = *reinterpret_cast<const Pack<T, VEC> *>(&v);
+  }
+  return r;
+}
+
+// VEC fp32 parameters (gamma, bias)
+template <int VEC>
+__device__ __forceinline__ void load_param(float (&o)[VEC], const float *p) {
+  if constexpr (VEC == 1) {
+    o[0] = __ldg(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + i));
+      o[i] = v.x;
+      o[i + 1] = v.y;
+      o[i + 2] = v.z;
+      o[i + 3] = v.w;
+    }
+  }
+}
+
+template <typename T, bool E4M3, int TPR, int VEC, int EPT>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rms_q8_kernel(RmsArgs a) {
+  constexpr int NV = EPT / VEC, ROWS = TPR == 32 ? 8 : 1;
+  __shared__ float red[64];
+  const long long row = (long long)blockIdx.x * ROWS + (TPR == 32 ? threadIdx.x / TPR : 0);
+  if (TPR == 32 && row >= a.n_rows) return;
+  const int t = threadIdx.x % TPR;
+  const int nc = a.D / VEC;   // chunks in a row (VEC > 1: D % VEC == 0)
+  const T *x = static_cast<const T *>(a.x) + row * a.D;
+  float v[EPT];
+  {
+    Pack<T, VEC> px[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if (t + j * TPR < nc) px[j] = load_pack<T, VEC, false>(x + (t + j * TPR) * VEC);
+    if (a.y) {
+      const T *y = static_cast<const T *>(a.y) + row * a.D;
+      Pack<T, VEC> py[NV];
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (t + j * TPR < nc) py[j] = load_pack<T, VEC, true>(y + (t + j * TPR) * VEC);
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (t + j * TPR < nc) {
+          float b[VEC];
+          if (a.bias) load_param<VEC>(b, a.bias + (t + j * TPR) * VEC);
+#pragma unroll
+          for (int i = 0; i < VEC; i++) {
+            float add = to_f32(py[j].e[i]);
+            if (a.bias) add = add + b[i];
+            px[j].e[i] = from_f32<T>(fmaf(add, a.alpha, to_f32(px[j].e[i])));
+          }
+        }
+    }
+    if (a.x_out) {
+      T *xo = static_cast<T *>(a.x_out) + row * a.D;
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (t + j * TPR < nc) *reinterpret_cast<Pack<T, VEC> *>(xo + (t + j * TPR) * VEC) = px[j];
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[j * VEC + i] = t + j * TPR < nc ? to_f32(px[j].e[i]) : 0.0f;
+  }
+  float ss = 0.0f, amax = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+    if (t + j * TPR < nc) {
+      float g[VEC];
+      load_param<VEC>(g, a.gamma + (t + j * TPR) * VEC);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        const float x1 = v[j * VEC + i];
+        ss = fmaf(x1, x1, ss);
+        v[j * VEC + i] = x1 * g[i];
+        amax = max_nan(amax, fabsf(v[j * VEC + i]));
+      }
+    }
+  row_reduce<TPR>(ss, amax, red);
+  float up;
+  const float mul = row_mul<E4M3>(ss, amax, up);
+  if (up != 1.0f) {
+#pragma unroll
+    for (int i = 0; i < EPT; i++) v[i] *= up;
+  }
+  unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+    if (t + j * TPR < nc) {
+      Pack<unsigned char, VEC> o = {};
+      if (mul != 0.0f) q8<E4M3, VEC>(v + j * VEC, mul, o.e);
+      *reinterpret_cast<Pack<unsigned char, VEC> *>(q + (t + j * TPR) * VEC) = o;
+    }
+  if (t == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
+}
+
+template <typename T, bool E4M3, int VEC, int TPR, int EPT>
+void rms_launch_as(const RmsArgs &a, cudaStream_t s) {
+  const long long grid = TPR == 32 ? (a.n_rows + 7) / 8 : a.n_rows;
+  rms_q8_kernel<T, E4M3, TPR, VEC, EPT><<<(unsigned)grid, TPR == 32 ? 256 : TPR, 0, s>>>(a);
+}
+
+// Eight entries per thread up to 2048-wide rows: 12000 x 1024 fp32 took 27.8 us
+// with 128 threads per row, 28.0 with 128 threads of 16 (D padded to 2048),
+// 28.7 with 64 of 16 and 30.7 with a warp of 32 (more registers, fewer rows in
+// flight per SM). Wider rows take 16 or 32 per thread: 4000 x 4096 fp32 35.8 us
+// with 256 of 16, 36.9 with 512 of 8; 2049 x 8192 fp32 37.9 with 512 of 16, 39.9
+// with 256 of 32, but bf16, whose chunks take half the registers, 35.8 and 32.8.
+template <typename T, bool E4M3, int VEC>
+void rms_launch_rows(const RmsArgs &a, cudaStream_t s) {
+  if (a.D <= 256) rms_launch_as<T, E4M3, VEC, 32, 8>(a, s);
+  else if (a.D <= 512) rms_launch_as<T, E4M3, VEC, 64, 8>(a, s);
+  else if (a.D <= 1024) rms_launch_as<T, E4M3, VEC, 128, 8>(a, s);
+  else if (a.D <= 2048) rms_launch_as<T, E4M3, VEC, 256, 8>(a, s);
+  else if (a.D <= 4096) rms_launch_as<T, E4M3, VEC, 256, 16>(a, s);
+  else if (VEC == 8) rms_launch_as<T, E4M3, VEC, 256, 32>(a, s);
+  else rms_launch_as<T, E4M3, VEC, 512, 16>(a, s);
+}
+
+template <typename T, bool E4M3>
+int rms_launch_q(const RmsArgs &a, cudaStream_t s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.x_out | (uintptr_t)a.bias | (uintptr_t)a.gamma;
+  const bool vec = a.D % VEC == 0 && (at & 15) == 0 && ((uintptr_t)a.q | (uintptr_t)a.ldq) % VEC == 0;
+  if (a.D > 8192) rms_q8_long_kernel<T, E4M3><<<(unsigned)a.n_rows, 256, 0, s>>>(a);
+  else if (vec) rms_launch_rows<T, E4M3, VEC>(a, s);
+  else rms_launch_rows<T, E4M3, 1>(a, s);
+  return pkcu_launch_status("pkcu_residual_rms_norm_q8");
 }
 
 template <typename T>
 int rms_launch(const RmsArgs &a, int e4m3, cudaStream_t s) {
-  if (e4m3) rms_q8_long_kernel<T, true><<<(unsigned)a.n_rows, 256, 0, s>>>(a);
-  else rms_q8_long_kernel<T, false><<<(unsigned)a.n_rows, 256, 0, s>>>(a);
-  return pkcu_launch_status("pkcu_residual_rms_norm_q8");
+  return e4m3 ? rms_launch_q<T, true>(a, s) : rms_launch_q<T, false>(a, s);
 }
 
 }  // namespace pk

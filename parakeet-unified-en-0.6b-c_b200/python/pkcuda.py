@@ -288,26 +288,30 @@ def _require(ok, what) -> None:
 
 
 def _vector(t, n, what):
-    """fp32 [n] on the GPU, packed (or None)."""
-    if t is not None:
-        import torch
-        _require(t.dtype == torch.float32 and t.is_cuda and t.is_contiguous() and t.numel() == n,
-                 f"{what}: a packed fp32 CUDA tensor of {n} entries is needed")
+    """fp32 [n], packed (or None)."""
+    if t is not None and not (dtype_of(t) == PKCU_DTYPE_F32 and t.is_contiguous() and t.numel() == n):
+        raise ValueError(f"{what}: a packed fp32 tensor of {n} entries is needed")
 
 
 def _call_on(t, stream, name, *args) -> None:
-    """call(name, *args, stream) on the device of t."""
+    """call(name, *args, stream) on the device of t; stream: a torch stream of
+    that device, None for its current one (read through torch's raw accessor:
+    torch.cuda.current_stream builds an object, 3 us a call)."""
     import torch
-    if t.device.index != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
-            call(name, *args, stream_handle(stream))
+    dev = t.get_device()
+    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            call(name, *args, raw)
     else:
-        call(name, *args, stream_handle(stream))
+        call(name, *args, raw)
 
 
 def _same_device(t, *others) -> None:
+    dev = t.get_device()
     for o in others:
-        _require(o is None or o.device == t.device, "tensors on different devices")
+        if o is not None and o.get_device() != dev:
+            raise ValueError("tensors on different devices")
 
 
 def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream=None) -> None:
@@ -316,9 +320,9 @@ def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream
     as in C."""
     _require(x.dim() == 2 and x.is_cuda and x.is_contiguous(), "x: a packed [n_rows, D] CUDA tensor is needed")
     rows, D = x.shape
-    for t, what in ((y, "y"), (x_out, "x_out")):
+    for t in (y, x_out):
         _require(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous()),
-                 f"{what}: the shape and type of x, packed, are needed")
+                 "y and x_out: the shape and type of x, packed, are needed")
     _require(q.dim() == 2 and q.shape[0] == rows and q.shape[1] >= D and (q.stride(1) == 1 or q.shape[1] == 1),
              "q: [n_rows, >= D] with packed columns is needed")
     _vector(gamma, D, "gamma")
