@@ -265,6 +265,10 @@ int pkcu_dequant_i4_qkv(const uint8_t *pq, const uint8_t *pk, const uint8_t *pv,
 
 #define PKCU_ACT_RELU 0   /* csrc/decoder.c:62-67 */
 #define PKCU_ACT_TANH 1
+/* the activations of pkcu_wmatmul_q8 alone (below) */
+#define PKCU_ACT_NONE  2
+#define PKCU_ACT_SWISH 3   /* v / (1 + exp(-v)) */
+#define PKCU_ACT_GELU  4   /* v (1 + erf(v / sqrt 2)) / 2 */
 /* Joint add + activation: out[b,t,j] = act(enc[b,t,j] + pred[b,j]). */
 int pkcu_joint_add_act(const float *enc, const float *pred, float *out, int B, int T, int J,
                        int act, pkcu_stream_t stream);
@@ -301,6 +305,31 @@ int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, f
                               const float *gamma, float eps, int dtype, void *x_out, void *q,
                               int qtype, long long ldq, float *scales, int n_rows, int D,
                               pkcu_stream_t stream);
+
+/* Products of 8-bit activations and 8-bit weights on the tcgen05 tensor cores,
+ * the bias, the activation and the residual in the epilogue:
+ *   C[m, n] = R[m, n] + rscale * act(a_scales[m] * w_scales[n] *
+ *                                    sum_k A[m, k] W[k, n] + bias[n])
+ * int8 x int8 summed exactly in 32-bit integers, e4m3 x e4m3 in fp32 (one
+ * rounding per 32 of K at most as coarse as fp32's); the rest in fp32, rounded once to
+ * C's type.
+ * A weight is prepared once (synchronous, on the current device): data [K, N]
+ * row-major device memory of type I8 (-127 .. 127 in the reference's
+ * checkpoints; -128 is taken as it is) or E4M3, scales fp32 device memory, 1
+ * for the whole weight (the reference's int8 storage) or N, one per column.
+ * K up to 131071; no divisibility is asked of K or N. */
+typedef struct pkcu_weight_q8 pkcu_weight_q8;
+int  pkcu_weight_q8_create(const void *data, int dtype, const float *scales, int n_scales, int K,
+                           int N, pkcu_stream_t stream, pkcu_weight_q8 **out);
+void pkcu_weight_q8_destroy(pkcu_weight_q8 *w);
+/* A [M, lda] bytes of the weight's type, K of each row used (lda a multiple of
+ * 16, A 16-byte aligned: pkcu_residual_rms_norm_q8 writes such rows), a_scales
+ * [M]; bias [N] or NULL; act PKCU_ACT_*; R [M, ldr] or NULL (nothing added) and
+ * C [M, ldc] of type dtype (F32, BF16 or F16), pitches in entries; R may be C.
+ * No work buffer; calls of one weight may run at the same time. */
+int  pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scales, const pkcu_weight_q8 *W,
+                     const float *bias, int act, const void *R, long long ldr, float rscale,
+                     void *C, long long ldc, int dtype, int M, pkcu_stream_t stream);
 
 /* ── 3. sequence driver ──────────────────────────────────────────────────── */
 

@@ -834,6 +834,13 @@ int launch(const CUtensorMap &ma, const CUtensorMap &mb, int M, int N, int K, co
 }
 }  // namespace
 
+extern "C" int pk_tensor_map_encoder(void **fn) {
+  PFN_cuTensorMapEncodeTiled_v12000 f = nullptr;
+  const int st = encoder_fn(&f);
+  *fn = reinterpret_cast<void *>(f);
+  return st;
+}
+
 extern "C" void pk_tc_warm(void) {
   smem_optin(tc::tc_gemm_kernel<1, 256>, tc::Cfg<1, 256>::SMEM, optin_flags<1, 256>());
   smem_optin(tc::tc_gemm_kernel<3, 256>, tc::Cfg<3, 256>::SMEM, optin_flags<3, 256>());

@@ -54,6 +54,10 @@ int pk_softmax_wait_timeouts(unsigned *count, int reset);
 int pk_conv_wait_timeouts(unsigned *count, int reset);
 int pk_tc_wait_timeouts(unsigned *count, int reset);   /* k_tcgemm.cu */
 
+int pk_q8_wait_timeouts(unsigned *count, int reset);   /* k_q8gemm.cu */
+/* The driver's cuTensorMapEncodeTiled (looked up once, k_tcgemm.cu). */
+int pk_tensor_map_encoder(void **fn);
+
 /* The library's tcgen05 GEMM (k_tcgemm.cu): C = epilogue(alpha * A W) with A
  * given as its three bf16 parts [M, 3K] (pk_split_rows_bf16x3) and W as
  * npb K-major bf16 planes [N, npb K] (pk_tc_prepare); K % 32 == 0, N % 32 == 0. */

@@ -19,7 +19,7 @@ CSRC_DIR = os.path.join(PKG_DIR, "csrc")
 D, H, DH, FF = 1024, 8, 128, 4096
 PKCU_CHANNEL_FIRST, PKCU_TIME_FIRST = 0, 1
 PKCU_GROUP_ALONG_K, PKCU_GROUP_ALONG_N = 0, 1
-PKCU_ACT_RELU, PKCU_ACT_TANH = 0, 1
+PKCU_ACT_RELU, PKCU_ACT_TANH, PKCU_ACT_NONE, PKCU_ACT_SWISH, PKCU_ACT_GELU = 0, 1, 2, 3, 4
 PKCU_DTYPE_F32, PKCU_DTYPE_I8, PKCU_DTYPE_I4 = 0, 1, 2
 PKCU_DTYPE_BF16, PKCU_DTYPE_F16, PKCU_DTYPE_E4M3 = 3, 4, 5
 PKCU_CHUNK_AUTO, PKCU_CHUNK_OFF, PKCU_CHUNK_ON = 0, 1, 2
@@ -67,6 +67,7 @@ EXPORTED = (
     "pkcu_wmatmul_bias_swish", "pkcu_wmatmul_bias_residual", "pkcu_wmatmul_qkv",
     "pkcu_encoder_nongemm_fused", "pkcu_conv_weight_create", "pkcu_pointwise_conv1d",
     "pkcu_pointwise_conv1d_glu", "pkcu_residual_rms_norm_q8",
+    "pkcu_weight_q8_create", "pkcu_weight_q8_destroy", "pkcu_wmatmul_q8",
 )
 
 
@@ -202,6 +203,9 @@ _SIGS = {
     "pkcu_conv_weight_create": (I, [VP, I, I, I, VP, C.POINTER(VP)]),
     "pkcu_pointwise_conv1d": (I, [VP, VP, VP, VP, I, VP, VP]),
     "pkcu_pointwise_conv1d_glu": (I, [VP, VP, VP, VP, I, VP, VP]),
+    "pkcu_weight_q8_create": (I, [VP, I, VP, I, I, I, VP, C.POINTER(VP)]),
+    "pkcu_weight_q8_destroy": (None, [VP]),
+    "pkcu_wmatmul_q8": (I, [VP, LL, VP, VP, VP, I, VP, LL, F, VP, LL, I, I, VP]),
     "pkcu_residual_rms_norm_q8": (I, [VP, VP, VP, F, VP, F, I, VP, VP, I, LL, VP, I, I, VP]),
 }
 
@@ -332,6 +336,71 @@ def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream
     _call_on(x, stream, "pkcu_residual_rms_norm_q8", x.data_ptr(), ptr(y), ptr(bias), alpha, gamma.data_ptr(),
              eps, dtype_of(x), ptr(x_out), q.data_ptr(), dtype_of(q), q.stride(0) if rows > 1 else max(q.stride(0), D),
              scales.data_ptr(), rows, D)
+
+
+class WeightQ8:
+    """pkcu_weight_q8: an int8 or e4m3 weight [K, N] prepared for wmatmul_q8;
+    scales: a tensor of 1 or N fp32 entries, or a number."""
+
+    def __init__(self, data, scales, stream=None):
+        import torch
+        self.handle = VP()
+        _require(data.dim() == 2 and data.is_cuda and data.is_contiguous(), "data: a packed [K, N] CUDA tensor is needed")
+        K, N = data.shape
+        if not torch.is_tensor(scales):
+            scales = torch.full((1,), float(scales), device=data.device)
+        _vector(scales, 1 if scales.numel() == 1 else N, "scales")
+        _same_device(data, scales)
+        dev = data.get_device()
+        with torch.cuda.device(dev):
+            raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+            h = VP()
+            call("pkcu_weight_q8_create", data.data_ptr(), dtype_of(data), scales.data_ptr(), scales.numel(), K, N,
+                 raw, C.byref(h))
+        self.handle, self.K, self.N, self.dtype = h, K, N, data.dtype
+
+    def close(self):
+        if self.handle:
+            lib().pkcu_weight_q8_destroy(self.handle)
+            self.handle = VP()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+_ACTS = {"relu": PKCU_ACT_RELU, "tanh": PKCU_ACT_TANH, "none": PKCU_ACT_NONE, None: PKCU_ACT_NONE,
+         "swish": PKCU_ACT_SWISH, "gelu": PKCU_ACT_GELU}
+
+
+def wmatmul_q8(a, a_scales, weight, out, bias=None, act=None, residual=None, rscale=1.0, stream=None) -> None:
+    """pkcu_wmatmul_q8 on tensors: a [M, >= K] of the weight's type (its row
+    pitch a multiple of 16), out and residual [M, N] with packed columns; act:
+    None, "relu", "tanh", "swish" or "gelu"."""
+    _require(weight.handle, "the weight is closed")
+    _require(a.dim() == 2 and a.is_cuda and a.dtype == weight.dtype and a.shape[1] >= weight.K and a.stride(1) == 1,
+             "a: [M, >= K] of the weight's type with packed columns is needed")
+    M = a.shape[0]
+    for t in (out, residual):
+        _require(t is None or (t.dim() == 2 and t.shape[0] == M and t.shape[1] == weight.N
+                               and (t.stride(1) == 1 or weight.N == 1) and t.dtype == out.dtype),
+                 "out and residual: [M, N] of one type with packed columns are needed")
+    _vector(a_scales, M, "a_scales")
+    _vector(bias, weight.N, "bias")
+    _same_device(a, a_scales, out, bias, residual)
+    lda = a.stride(0) if M > 1 else (a.shape[1] + 15) // 16 * 16
+    ldc = out.stride(0) if M > 1 else max(out.stride(0), weight.N)
+    ldr = 0 if residual is None else residual.stride(0) if M > 1 else max(residual.stride(0), weight.N)
+    _call_on(a, stream, "pkcu_wmatmul_q8", a.data_ptr(), lda, a_scales.data_ptr(), weight.handle, ptr(bias),
+             _ACTS[act], ptr(residual), ldr, rscale, out.data_ptr(), ldc, dtype_of(out), M)
 
 
 class Seq:

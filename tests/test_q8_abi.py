@@ -33,3 +33,23 @@ def test_rms_norm_refusals(L, change, word):
     assert L.pkcu_residual_rms_norm_q8(*a.values(), None) == ERR_ARG
     msg = L.pkcu_last_error().decode()
     assert "pkcu_residual_rms_norm_q8" in msg and word in msg, msg
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(dtype=0), "type"), (dict(dtype=3), "type"), (dict(K=0), "K 0"), (dict(K=131072), "K"), (dict(N=0), "N 0"),
+    (dict(n_scales=2), "scales"), (dict(n_scales=0), "scales"), (dict(data=None), "NULL"),
+    (dict(scales=None), "NULL"), (dict(scales=P + 2), "aligned")])
+def test_weight_q8_refusals(L, change, word):
+    h = C.c_void_p(7)
+    a = dict(data=P, dtype=1, scales=P, n_scales=64, K=64, N=64)
+    a.update(change)
+    assert L.pkcu_weight_q8_create(*a.values(), None, C.byref(h)) == ERR_ARG
+    msg = L.pkcu_last_error().decode()
+    assert "pkcu_weight_q8_create" in msg and word in msg and not h.value, msg
+    assert L.pkcu_weight_q8_create(*a.values(), None, None) == ERR_ARG
+    L.pkcu_weight_q8_destroy(None)
+
+
+def test_product_needs_a_weight(L):
+    assert L.pkcu_wmatmul_q8(P, 64, P, None, None, 2, None, 0, 1.0, P, 64, 0, 4, None) == ERR_ARG
+    assert b"NULL weight" in L.pkcu_last_error()
