@@ -208,7 +208,7 @@ def _act(v, act):
 
 def _product(s):
     if own:
-        _lib().wmatmul_q8(s["a"], s["a_scales"], s["weight"], s["out"], bias=s["b"], act=s["act"], residual=s["r"], rscale=0.5)
+        _lib().wmatmul_q8(s["a"], s["a_scales"], s["weight"], s["out"], bias=s["b"], act=s["act"], residual=s["r"], rscale=0.5 if s["residual"] else 1.0)
         return s["out"]
     v = (s["a"][:, :s["k"]].float() @ s["w"].float()) * s["a_scales"][:, None] * s["w_scales"][None, :]
     if s["b"] is not None:
