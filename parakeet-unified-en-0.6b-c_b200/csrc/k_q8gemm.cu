@@ -58,6 +58,7 @@ struct Args {
   float rscale;
   int act, dtype;
   int M, N, nkb;
+  int r_vec, c_vec;   // rows of R / C 16-byte aligned
 };
 
 // ── PTX wrappers ──────────────────────────────────────────────────────────────
@@ -69,6 +70,10 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, i
       " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
+}
+
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(map)) : "memory");
 }
 
 // Shared-memory matrix descriptor: K-major rows of 128 bytes, 128-byte swizzle,
@@ -160,19 +165,23 @@ __device__ __forceinline__ void tmem_ld(unsigned taddr, unsigned (&r)[NC]) {
 
 // ── epilogue ──────────────────────────────────────────────────────────────────
 
-// Tokens m .. m + NC - 1 of output n, from their sums; sa: this lane's a_scales
-// entry (lane j holds token m + j's). Runs on whole warps; a lane past N only
-// lends its scale.
-template <bool E4M3, int NC, typename T>
-__device__ __forceinline__ void finish(const Args &a, int m, int n, float sw, float bias, float sa,
-                                       const unsigned (&acc)[NC]) {
-  float v[NC];
-#pragma unroll
-  for (int j = 0; j < NC; j++) {
-    const float s = E4M3 ? __uint_as_float(acc[j]) : __int2float_rn((int)acc[j]);
-    v[j] = fmaf(s * sw, __shfl_sync(PK_FULL_MASK, sa, j), bias);
-  }
-  switch (a.act) {
+// v / (1 + exp(-v)) on a pair: exp(-v) = 2^-h (1 + l ln 2) with h the rounded
+// product v log2 e and -l the rest of the exact one, 2^-h and the reciprocal by
+// the hardware's approximations (2 and 1 units in the last place); past 2^125
+// (v below -86) the power stands still and the result is below 1e-35.
+__device__ __forceinline__ float2 swish_ex2(float2 v) {
+  const float2 h = mul2(v, splat2(GATE_L2E_HI));
+  float2 l = fma2(v, splat2(-GATE_L2E_HI), h);
+  l = mul2(fma2(v, splat2(-GATE_L2E_LO), l), splat2(0.693147180559945f));
+  float2 e = make_float2(ex2_approx(fminf(-h.x, 125.0f)), ex2_approx(fminf(-h.y, 125.0f)));
+  e = fma2(e, l, e);
+  const float2 d = add2(splat2(1.0f), e);
+  return mul2(v, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+}
+
+template <int NC>
+__device__ __forceinline__ void activate(int act, float (&v)[NC]) {
+  switch (act) {
     case PKCU_ACT_RELU:
 #pragma unroll
       for (int j = 0; j < NC; j++) v[j] = v[j] < 0.0f ? 0.0f : v[j];
@@ -184,7 +193,7 @@ __device__ __forceinline__ void finish(const Args &a, int m, int n, float sw, fl
     case PKCU_ACT_SWISH:
 #pragma unroll
       for (int j = 0; j < NC; j += 2) {
-        const float2 s = glu_gate2(make_float2(v[j], v[j + 1]), make_float2(v[j], v[j + 1]), splat2(-0.0f));
+        const float2 s = swish_ex2(make_float2(v[j], v[j + 1]));
         v[j] = s.x;
         v[j + 1] = s.y;
       }
@@ -195,32 +204,59 @@ __device__ __forceinline__ void finish(const Args &a, int m, int n, float sw, fl
       break;
     default: break;
   }
+}
+
+template <bool E4M3>
+__device__ __forceinline__ float sum_as_float(unsigned acc) {
+  return E4M3 ? __uint_as_float(acc) : __int2float_rn((int)acc);
+}
+
+// Tokens m .. m + NC - 1 of output n, from their sums; sa: this lane's a_scales
+// entry (lane j holds token m + j's). Runs on whole warps; a lane past N only
+// lends its scale.
+template <bool E4M3, int NC, typename T>
+__device__ __forceinline__ void finish(const Args &a, int m, int n, float sw, float bias, float sa,
+                                       const unsigned (&acc)[NC]) {
+  float v[NC];
+#pragma unroll
+  for (int j = 0; j < NC; j++)
+    v[j] = fmaf(sum_as_float<E4M3>(acc[j]) * sw, __shfl_sync(PK_FULL_MASK, sa, j), bias);
+  activate<NC>(a.act, v);
   if (n >= a.N) return;
   const int nm = a.M - m < NC ? a.M - m : NC;
   if (a.R) {
     const T *r = static_cast<const T *>(a.R) + (long long)m * a.ldr + n;
     T x[NC];
 #pragma unroll
-    for (int j = 0; j < NC; j++)
-      if (j < nm) x[j] = r[(long long)j * a.ldr];
+    for (int j = 0; j < NC; j++, r += a.ldr)
+      if (j < nm) x[j] = *r;
 #pragma unroll
     for (int j = 0; j < NC; j++)
       if (j < nm) v[j] = fmaf(v[j], a.rscale, to_f32(x[j]));
-  } else if (a.rscale != 1.0f) {
+  } else {
 #pragma unroll
     for (int j = 0; j < NC; j++) v[j] *= a.rscale;
   }
   T *c = static_cast<T *>(a.C) + (long long)m * a.ldc + n;
+  if (nm == NC) {
 #pragma unroll
-  for (int j = 0; j < NC; j++)
-    if (j < nm) c[(long long)j * a.ldc] = from_f32<T>(v[j]);
+    for (int j = 0; j < NC; j++, c += a.ldc) *c = from_f32<T>(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NC; j++, c += a.ldc)
+      if (j < nm) *c = from_f32<T>(v[j]);
+  }
 }
 
-template <bool E4M3, int NC>
-__device__ __forceinline__ void finish_any(const Args &a, int m, int n, float sw, float bias,
-                                           const unsigned (&acc)[NC]) {
+// Lane j < NC: the scale of token m + j.
+template <int NC>
+__device__ __forceinline__ float token_scale(const Args &a, int m) {
   const int lane = threadIdx.x & 31;
-  const float sa = lane < NC && m + lane < a.M ? __ldg(a.a_scales + m + lane) : 0.0f;
+  return lane < NC && m + lane < a.M ? __ldg(a.a_scales + m + lane) : 0.0f;
+}
+template <bool E4M3, int NC>
+__device__ __forceinline__ void finish_any(const Args &a, int m, int n, float sw, float bias, float sa,
+                                           const unsigned (&acc)[NC]) {
   if (a.dtype == PKCU_DTYPE_F32) finish<E4M3, NC, float>(a, m, n, sw, bias, sa, acc);
   else if (a.dtype == PKCU_DTYPE_BF16) finish<E4M3, NC, __nv_bfloat16>(a, m, n, sw, bias, sa, acc);
   else finish<E4M3, NC, __half>(a, m, n, sw, bias, sa, acc);
@@ -256,7 +292,17 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const long long tile0 = SPLIT ? blockIdx.x / split : blockIdx.x;
   const long long step = SPLIT ? n_tiles : gridDim.x;
 
+  // the first tile's loads are on their way before anything else is set up
+  const int first_kb = kb1 - kb0 < C::STAGES ? kb1 - kb0 : C::STAGES;
+  auto load_stage = [&](int s, int kb, int n0, int m0) {
+    unsigned char *st = smem + s * C::STAGE;
+    mbar_arrive_tx(full + s, C::STAGE);
+    tma_load_2d(st, &map_w, kb * BK, n0, full + s);
+    tma_load_2d(st + W_TILE, &map_a, kb * BK, m0, full + s);
+  };
   if (threadIdx.x == 0) {
+    tma_prefetch_map(&map_w);
+    tma_prefetch_map(&map_a);
     for (int s = 0; s < C::STAGES; s++) {
       mbar_init(full + s, 1);
       mbar_init(empty + s, 1);
@@ -268,6 +314,8 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     mbar_init(done, 1);
     mbar_init_fence();
     s_abort = 0;
+    for (int i = 0; i < first_kb; i++)
+      load_stage(i, kb0 + i, (int)(tile0 / tiles_m) * BP, (int)(tile0 % tiles_m) * BQ);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -283,11 +331,11 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
   if (warp == 0) {
     if (lane == 0) {
-      long long it = 0;   // stages filled by this CTA, over all its tiles
+      long long it = first_kb;   // stages filled by this CTA, over all its tiles
       bool stop = false;
       for (long long tile = tile0; tile < n_tiles && !stop; tile += step) {
         const int n0 = (int)(tile / tiles_m) * BP, m0 = (int)(tile % tiles_m) * BQ;
-        for (int kb = kb0; kb < kb1; kb++, it++) {
+        for (int kb = tile == tile0 ? kb0 + first_kb : kb0; kb < kb1; kb++, it++) {
           const int s = (int)(it % C::STAGES);
           if (it >= C::STAGES && !mbar_wait(empty + s, (unsigned)((it / C::STAGES) - 1) & 1)) {
             atomicAdd(&g_wait_timeouts, 1u);
@@ -297,10 +345,7 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             stop = true;
             break;
           }
-          unsigned char *st = smem + s * C::STAGE;
-          mbar_arrive_tx(full + s, C::STAGE);
-          tma_load_2d(st, &map_w, kb * BK, n0, full + s);
-          tma_load_2d(st + W_TILE, &map_a, kb * BK, m0, full + s);
+          load_stage(s, kb, n0, m0);
         }
       }
       if (*(volatile int *)&s_abort) {
@@ -355,6 +400,7 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const int buf = gt & 1, n = n0 + q * 32 + lane;
       const float sw = n < a.N ? __ldg(a.w_scales + n) : 0.0f;
       const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+      float sa = SPLIT ? 0.0f : token_scale<C::CH>(a, m0 + half * C::CW);
       // the outcome is made warp-uniform: tcgen05.ld needs every lane
       if (!__all_sync(PK_FULL_MASK, mbar_wait(acc_full + buf, (gt >> 1) & 1))) {
         if (lane == 0) atomicAdd(&g_wait_timeouts, 1u);
@@ -374,7 +420,9 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           for (int j = 0; j < C::CH; j++) part[(half * C::CW + c + j) * BP + q * 32 + lane] = r[j];
         } else {
           const int m = m0 + half * C::CW + c;
-          if (m < a.M) finish_any<E4M3, C::CH>(a, m, n, sw, bias, r);
+          const float now = sa;
+          if (c + C::CH < C::CW) sa = token_scale<C::CH>(a, m + C::CH);
+          if (m < a.M) finish_any<E4M3, C::CH>(a, m, n, sw, bias, now, r);
         }
       }
       tc_fence_before();
@@ -383,16 +431,17 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     }
   }
   if constexpr (SPLIT) {
+    // columns (tokens) 8 i .. 8 i + 7 go to rank i mod S, a warp of each
+    // quadrant of n; sums in rank order
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int n0 = (int)(tile0 / tiles_m) * BP, m0 = (int)(tile0 % tiles_m) * BQ;
+    const int n = n0 + q * 32 + lane;
+    const float sw = n < a.N ? __ldg(a.w_scales + n) : 0.0f;
+    const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+    float sa = warp >= 2 ? token_scale<8>(a, m0 + (rank + half * split) * 8) : 0.0f;
     __syncwarp();
     cluster_sync_all();   // every rank's partial sums are in its shared memory
     if (warp >= 2 && !*(volatile int *)&s_abort) {
-      // columns (tokens) 8 i .. 8 i + 7 go to rank i mod S, a warp of each
-      // quadrant of n; sums in rank order
-      const int q = warp & 3, half = (warp - 2) >> 2;
-      const int n0 = (int)(tile0 / tiles_m) * BP, m0 = (int)(tile0 % tiles_m) * BQ;
-      const int n = n0 + q * 32 + lane;
-      const float sw = n < a.N ? __ldg(a.w_scales + n) : 0.0f;
-      const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
       const unsigned base = smem_u32(smem);
       for (int g = rank + half * split; g < BQ / 8; g += 2 * split) {
         if (m0 + g * 8 >= a.M) break;
@@ -407,7 +456,8 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           for (int j = 0; j < 8; j++)
             r[j] = E4M3 ? __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(t[j])) : r[j] + t[j];
         }
-        finish_any<E4M3, 8>(a, m0 + g * 8, n, sw, bias, r);
+        finish_any<E4M3, 8>(a, m0 + g * 8, n, sw, bias, sa, r);
+        sa = token_scale<8>(a, m0 + (g + 2 * split) * 8);
       }
     }
     __syncwarp();
@@ -418,6 +468,381 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS)
+                 : "memory");
+  }
+}
+
+// ── many tokens: CTA pairs, rows of C by TMA ─────────────────────────────────
+//
+// One 256-token x BN-output tile per pair of CTAs (tcgen05 cta_group::2): each CTA
+// brings 128 tokens and half of the outputs' weight rows, the pair's MMA reads both
+// CTAs' shared memory, and each CTA's TMEM holds its 128 tokens x BN sums. So a
+// CTA loads (128 + BN / 2) bytes per byte of K for 128 x BN products: two thirds
+// of what a single CTA's 128 x 256 tile loads, which is what the L2 could not
+// deliver at the 8-bit MMA rate.
+//
+// Here a TMEM lane is a token and its columns are outputs: a thread turns 32
+// columns into 128 (or 64) consecutive bytes of its row with the scale of its
+// token in a register, writes them to a swizzled 32-row buffer of its warp with
+// 16-byte stores, and a TMA store of the box takes them to C: about 6
+// instructions per output besides the activation, against 26 for one store per
+// output and token. C must suit TMA (16-byte aligned rows).
+
+#ifndef PEPI
+#define PEPI 8
+#endif
+constexpr int PAIR_EPI = PEPI;
+constexpr int PAIR_THREADS = 32 * (2 + PAIR_EPI);
+struct PairCfg {
+  static constexpr int BN = 256;
+  static constexpr int A_TILE = 128 * BK, B_TILE = BN / 2 * BK;
+  static constexpr int STAGE = A_TILE + B_TILE;
+  static constexpr int OUT = PAIR_EPI * 4096;       // a 32-row x 128-byte box per epilogue warp
+  static constexpr int PAR = BN * 8;                 // scale and bias of the tile's outputs
+  static constexpr int REST = OUT + PAR + 256;
+  static constexpr int STAGES = (227 * 1024 - REST) / STAGE < 8 ? (227 * 1024 - REST) / STAGE : 8;
+  static constexpr int SMEM = STAGES * STAGE + REST;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int CW = BN / (PAIR_EPI / 4);   // columns per epilogue warp
+};
+
+__device__ __forceinline__ unsigned mapa(unsigned saddr, unsigned rank) {
+  unsigned a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+  return a;
+}
+// A load into this CTA's shared memory that reports to a barrier of either CTA
+// of the pair (bar: a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+template <bool E4M3>
+__device__ __forceinline__ void umma_pair(unsigned tmem_d, unsigned long long a, unsigned long long b, unsigned desc,
+                                          unsigned accumulate) {
+  if constexpr (E4M3)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+        : "memory");
+}
+// The barrier at this address in both CTAs, once the MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(unsigned long long *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((unsigned short)3)
+      : "memory");
+}
+// Relaxed: what it announces is that TMEM reads are done (waited for before).
+// A release would also wait for the stores to C in flight, 3000 cycles a tile.
+__device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// TMEM columns without waiting; tmem_wait() before the first use.
+__device__ __forceinline__ void tmem_ld32_async(unsigned taddr, unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// The registers pass through, so that no use moves above the wait.
+__device__ __forceinline__ void tmem_wait(unsigned (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// 32 entries n .. n + 31 of a row of R as raw 16-byte words (r NULL: none).
+template <typename T>
+struct RowChunk {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  float4 raw[32 / VEC];
+  __device__ __forceinline__ void load(const Args &a, const T *r, int n) {
+    if (!r) return;
+    if (a.r_vec && n + 32 <= a.N) {
+#pragma unroll
+      for (int i = 0; i < 32 / VEC; i++) raw[i] = *reinterpret_cast<const float4 *>(r + n + i * VEC);
+    } else {
+      T *e = reinterpret_cast<T *>(raw);
+#pragma unroll
+      for (int j = 0; j < 32; j++) e[j] = n + j < a.N ? r[n + j] : from_f32<T>(0.0f);
+    }
+  }
+};
+
+// 32 sums of this thread's token with scales and bias. par: for each pair of
+// outputs the two scales and the two biases, in shared memory, the same for
+// every lane.
+template <bool E4M3>
+__device__ __forceinline__ void scale_row(const float4 *par, float sa, const unsigned (&acc)[32], float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const float4 p = par[j / 2];
+    const float2 s = mul2(make_float2(sum_as_float<E4M3>(acc[j]), sum_as_float<E4M3>(acc[j + 1])), splat2(sa));
+    const float2 o = fma2(s, make_float2(p.x, p.y), make_float2(p.z, p.w));
+    v[j] = o.x;
+    v[j + 1] = o.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add_residual_row(const Args &a, bool resid, const RowChunk<T> &rc, float (&v)[32]) {
+  if (resid) {
+    const T *x = reinterpret_cast<const T *>(rc.raw);
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = fmaf(v[j], a.rscale, to_f32(x[j]));
+  } else if (a.rscale != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] *= a.rscale;
+  }
+}
+
+// 32 finished outputs as chunks 16 bytes wide of this lane's row of the box.
+template <typename T>
+__device__ __forceinline__ void box_row(unsigned char *box, int first, const float (&v)[32]) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; j += VEC) {
+    alignas(16) T o[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; i++) o[i] = from_f32<T>(v[j + i]);
+    const int chunk = (first + j) / VEC;   // chunk c of row r lies at c ^ (r mod 8): no bank conflicts
+    *reinterpret_cast<uint4 *>(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(o);
+  }
+}
+
+// The box (32 tokens from m0, 128 bytes of outputs from n0) to C: a store of the
+// warp covers four rows, 128 bytes of each.
+template <typename T>
+__device__ __forceinline__ void box_store(const Args &a, const unsigned char *box, int m0, int n0) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31, chunk = lane & 7;
+  const int n = n0 + chunk * VEC;
+  T *c = static_cast<T *>(a.C) + (long long)(m0 + (lane >> 3)) * a.ldc + n;
+  const bool whole = a.c_vec && n + VEC <= a.N;
+#pragma unroll
+  for (int i = 0; i < 8; i++, c += 4 * a.ldc) {
+    const int row = 4 * i + (lane >> 3);
+    const uint4 d = *reinterpret_cast<const uint4 *>(box + row * 128 + ((chunk ^ (row & 7)) << 4));
+    if (m0 + row < a.M) {
+      if (whole) {
+        *reinterpret_cast<uint4 *>(c) = d;
+      } else {
+        const T *e = reinterpret_cast<const T *>(&d);
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          if (n + j < a.N) c[j] = e[j];
+      }
+    }
+  }
+}
+
+template <bool E4M3, typename T>
+__global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
+q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, Args a) {
+  using C = PairCfg;
+  constexpr int BN = C::BN;
+  // the same offsets in both CTAs: an MMA's descriptors serve both
+  extern __shared__ __align__(1024) unsigned char pair_smem[];
+  unsigned char *smem = pair_smem;
+  unsigned char *out = smem + C::STAGES * C::STAGE;
+  float *par = reinterpret_cast<float *>(out + C::OUT);   // [BN / 2] x {scale, scale, bias, bias}
+  unsigned long long *full = reinterpret_cast<unsigned long long *>(out + C::OUT + C::PAR);   // the leader's is used
+  unsigned long long *empty = full + C::STAGES;
+  unsigned long long *acc_full = empty + C::STAGES;    // [2]
+  unsigned long long *acc_empty = acc_full + 2;        // [2], the leader's is used
+  unsigned long long *done = acc_empty + 2;
+  unsigned *tmem_slot = reinterpret_cast<unsigned *>(done + 1);
+  int &s_abort = *reinterpret_cast<int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned rank = blockIdx.x & 1;   // clusters of two consecutive CTAs; rank 0 leads
+  const int tiles_m = (a.M + 255) / 256;
+  const long long n_tiles = (long long)tiles_m * ((a.N + BN - 1) / BN);
+  const long long step = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&map_w);
+    tma_prefetch_map(&map_a);
+    for (int s = 0; s < C::STAGES; s++) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(acc_full + b, 1);
+      mbar_init(acc_empty + b, 2 * PAIR_EPI);
+    }
+    mbar_init(done, 1);
+    mbar_init_fence();
+    s_abort = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // both CTAs' barriers and TMEM exist before either signals or fills the other's
+  tc_fence_after();
+  const unsigned tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      long long it = 0;
+      bool stop = false;
+      for (long long tile = blockIdx.x >> 1; tile < n_tiles && !stop; tile += step) {
+        const int m0 = (int)(tile % tiles_m) * 256 + (int)rank * 128;
+        const int n0 = (int)(tile / tiles_m) * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < a.nkb; kb++, it++) {
+          const int s = (int)(it % C::STAGES);
+          if (it >= C::STAGES && !mbar_wait(empty + s, (unsigned)((it / C::STAGES) - 1) & 1)) {
+            atomicAdd(&g_wait_timeouts, 1u);
+            s_abort = 1;
+          }
+          if (*(volatile int *)&s_abort) {
+            stop = true;
+            break;
+          }
+          // the leader's barrier counts the bytes of both CTAs; a peer's bytes that
+          // land before its expect-tx leave the phase open all the same
+          if (rank == 0) mbar_arrive_tx(full + s, 2 * C::STAGE);
+          const unsigned st = smem_u32(smem + s * C::STAGE), bar = mapa(smem_u32(full + s), 0);
+          tma_load_2d_pair(st, &map_a, kb * BK, m0, bar);
+          tma_load_2d_pair(st + C::A_TILE, &map_w, kb * BK, n0, bar);
+        }
+      }
+      if (rank == 0 && *(volatile int *)&s_abort) {
+        for (long long j = it > C::STAGES ? it - C::STAGES : 0; j < it; j++)
+          mbar_wait(full + j % C::STAGES, (unsigned)(j / C::STAGES) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr unsigned DESC = idesc(E4M3, 256, BN);
+      long long it = 0;
+      int gt = 0;
+      for (long long tile = blockIdx.x >> 1; tile < n_tiles && !*(volatile int *)&s_abort; tile += step, gt++) {
+        const int buf = gt & 1;
+        if (gt >= 2 && !mbar_wait(acc_empty + buf, ((gt >> 1) - 1) & 1)) {
+          atomicAdd(&g_wait_timeouts, 1u);
+          s_abort = 1;
+          break;
+        }
+        tc_fence_after();
+        const unsigned d = tmem + buf * BN;
+        for (int kb = 0; kb < a.nkb; kb++, it++) {
+          const int s = (int)(it % C::STAGES);
+          if (!mbar_wait(full + s, (unsigned)(it / C::STAGES) & 1)) {
+            atomicAdd(&g_wait_timeouts, 1u);
+            s_abort = 1;
+            break;
+          }
+          tc_fence_after();
+          const unsigned st = smem_u32(smem + s * C::STAGE);
+#pragma unroll
+          for (int k = 0; k < BK / 32; k++)
+            umma_pair<E4M3>(d, sdesc_k128(st + k * 32), sdesc_k128(st + C::A_TILE + k * 32), DESC, kb > 0 || k > 0);
+          umma_commit_pair(empty + s);
+        }
+        if (*(volatile int *)&s_abort) break;
+        umma_commit_pair(acc_full + buf);
+      }
+      umma_commit_pair(done);
+      mbar_wait(done, 0);
+    }
+  } else {
+    // warp w: tokens 32 (w % 4) .. + 31 of this CTA's 128, half of the columns
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const unsigned lane_addr = ((unsigned)(q * 32) << 16) + half * C::CW;
+    unsigned char *box = out + (warp - 2) * 4096;
+    float *my_par = par + half * C::CW * 2;   // shared by the four warps of this half
+    constexpr int COLS = 128 / (int)sizeof(T);   // outputs per box
+    int gt = 0;
+    bool ok = true;   // after a wait that ran out a warp only keeps the others' barriers going
+    for (long long tile = blockIdx.x >> 1; tile < n_tiles; tile += step, gt++) {
+      const int m0 = (int)(tile % tiles_m) * 256 + (int)rank * 128 + q * 32;
+      const int n0 = (int)(tile / tiles_m) * BN + half * C::CW;
+      const int m = m0 + lane, buf = gt & 1;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");   // the last tile's pairs are read
+      for (int i = q * 32 + lane; i < C::CW; i += 128) {
+        const int n = n0 + i, at = (i & ~1) * 2 + (i & 1);
+        my_par[at] = n < a.N ? __ldg(a.w_scales + n) : 0.0f;
+        my_par[at + 2] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+      }
+      const float sa = m < a.M ? __ldg(a.a_scales + m) : 0.0f;
+      const T *r = a.R && m < a.M ? static_cast<const T *>(a.R) + (long long)m * a.ldr : nullptr;
+      RowChunk<T> rc;
+      rc.load(a, n0 < a.N ? r : nullptr, n0);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+      if (ok && !__all_sync(PK_FULL_MASK, mbar_wait(acc_full + buf, (gt >> 1) & 1))) {
+        if (lane == 0) atomicAdd(&g_wait_timeouts, 1u);
+        s_abort = 1;
+        ok = false;
+      }
+      if (!ok) continue;
+      tc_fence_after();
+      // 32 columns at a time; the next ones' TMEM load is in flight while the
+      // activation and the store of these go on, and their residual after it
+      unsigned acc[32];
+      const unsigned t0 = tmem + lane_addr + buf * BN;
+      tmem_ld32_async(t0, acc);
+      const float4 *p4 = reinterpret_cast<const float4 *>(my_par);
+#pragma unroll 1
+      for (int c = 0; c < C::CW; c += 32) {
+        float v[32];
+        tmem_wait(acc);
+        scale_row<E4M3>(p4 + c / 2, sa, acc, v);
+        if (c + 32 < C::CW) {
+          tmem_ld32_async(t0 + c + 32, acc);
+        } else {   // this warp's last sums are in registers: the accumulator may be filled again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(acc_empty + buf), 0));
+        }
+        activate<32>(a.act, v);
+        add_residual_row<T>(a, r != nullptr, rc, v);
+        if (c + 32 < C::CW) rc.load(a, n0 + c + 32 < a.N ? r : nullptr, n0 + c + 32);
+        const int first = c & (COLS - 1);   // this chunk's place in its box
+        box_row<T>(box, first, v);
+        if (first + 32 == COLS) {
+          __syncwarp();
+          if (n0 + c - first < a.N) box_store<T>(a, box, m0, n0 + c - first);
+          __syncwarp();
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  // no CTA leaves (or frees its TMEM) while the pair's MMAs, loads or signals may reach it
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS)
                  : "memory");
   }
 }
@@ -507,15 +932,66 @@ int launch(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, in
   return pkcu_launch_status("pkcu_wmatmul_q8");
 }
 
+template <bool E4M3, typename T>
+int launch_pair(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, cudaStream_t s) {
+  using C = q8::PairCfg;
+  static int flags[64];
+  smem_optin(q8::q8_pair_kernel<E4M3, T>, C::SMEM, flags);
+  const long long tiles = (long long)((a.M + 255) / 256) * ((a.N + C::BN - 1) / C::BN);
+  const long long pairs = pkcu_sm_count() / 2;
+  const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
+  q8::q8_pair_kernel<E4M3, T><<<grid, q8::PAIR_THREADS, C::SMEM, s>>>(W->map, ma, a);
+  return pkcu_launch_status("pkcu_wmatmul_q8");
+}
+
+int launch_pair_any(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, cudaStream_t s) {
+  if (a.dtype == PKCU_DTYPE_F32) return W->e4m3 ? launch_pair<true, float>(W, ma, a, s) : launch_pair<false, float>(W, ma, a, s);
+  if (a.dtype == PKCU_DTYPE_BF16)
+    return W->e4m3 ? launch_pair<true, __nv_bfloat16>(W, ma, a, s) : launch_pair<false, __nv_bfloat16>(W, ma, a, s);
+  return W->e4m3 ? launch_pair<true, __half>(W, ma, a, s) : launch_pair<false, __half>(W, ma, a, s);
+}
+
 template <bool E4M3, bool SPLIT>
 int launch_bq(int bq, const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, int split, cudaStream_t s) {
   switch (bq) {
     case 16: return launch<E4M3, 16, SPLIT>(W, ma, a, split, s);
     case 32: return launch<E4M3, 32, SPLIT>(W, ma, a, split, s);
     case 64: return launch<E4M3, 64, SPLIT>(W, ma, a, split, s);
-    case 128: return launch<E4M3, 128, SPLIT>(W, ma, a, split, s);
-    default: return launch<E4M3, 256, false>(W, ma, a, split, s);
+    default: return launch<E4M3, 128, SPLIT>(W, ma, a, split, s);
   }
+}
+
+constexpr int PAIR = 256;   // the pair kernel's tokens per tile
+struct Plan {
+  int bq, split;
+};
+// DISPATCH-COMMENT
+Plan plan(int M, int N, int nkb, int sms) {
+  const char *e1 = getenv("BQ"), *e2 = getenv("SMAX");
+  if (e1) {
+    Plan p = {atoi(e1), e2 ? atoi(e2) : 1};
+    return p;
+  }
+  static const float fixed_us[5] = {3.3f, 4.0f, 5.0f, 7.0f, 8.9f};
+  Plan best = {PAIR, 1};
+  float best_us = INFINITY;
+  const long long tiles_n = ((long long)N + q8::BP - 1) / q8::BP;
+  for (int i = 0; i < 5; i++) {
+    const int bq = 16 << i;
+    const bool pair = bq == PAIR;
+    const long long tiles = ((long long)M + bq - 1) / bq * (pair ? ((long long)N + 255) / 256 : tiles_n);
+    const long long slots = pair ? sms / 2 : sms;
+    for (int split = 1; split <= (pair ? 1 : 8) && split <= nkb && (split == 1 || tiles * split <= sms); split *= 2) {
+      const float waves = (float)((tiles * split + slots - 1) / slots);
+      const float us = fixed_us[i] + (split > 1 ? 2.0f + 0.2f * split : 0.0f) + waves * (float)((nkb + split - 1) / split) * 0.34f;
+      if (us < best_us) {
+        best_us = us;
+        best.bq = bq;
+        best.split = split;
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -618,17 +1094,14 @@ extern "C" int pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scal
   a.M = M;
   a.N = W->N;
   a.nkb = (W->K + q8::BK - 1) / q8::BK;
-  const int sms = pkcu_sm_count();
-  const long long tiles_n = (W->N + q8::BP - 1) / q8::BP;
-  int bq = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  while (bq > 64 && tiles_n * ((M + bq - 1) / bq) * 2 < sms) bq >>= 1;
-  const long long tiles = tiles_n * ((M + bq - 1) / bq);
-  int split = 1;
-  if (bq <= 128)
-    while (split < 8 && tiles * split * 2 <= sms && split * 2 <= a.nkb) split *= 2;
+  a.r_vec = PK_ALIGNED16(R) && ldr * size % 16 == 0;
+  a.c_vec = PK_ALIGNED16(C) && ldc * size % 16 == 0;
+  const Plan p = plan(M, W->N, a.nkb, pkcu_sm_count());
   CUtensorMap ma;
-  const int st = tmap_bytes(&ma, A, M, W->K, lda, bq);
+  const int st = tmap_bytes(&ma, A, M, W->K, lda, p.bq == PAIR ? 128 : p.bq);
   if (st) return st;
+  if (p.bq == PAIR) return launch_pair_any(W, ma, a, (cudaStream_t)stream);
+  const int bq = p.bq, split = p.split;
   cudaStream_t s = (cudaStream_t)stream;
   if (split > 1)
     return W->e4m3 ? launch_bq<true, true>(bq, W, ma, a, split, s) : launch_bq<false, true>(bq, W, ma, a, split, s);
