@@ -124,6 +124,13 @@ __device__ __forceinline__ void tc_fence_after() {
 __device__ __forceinline__ void mbar_arrive(unsigned long long *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// One lane polls for its warp (32 would take issue slots and shared-memory cycles
+// from the warps at work); the outcome is warp-uniform, as tcgen05.ld needs it.
+__device__ __forceinline__ bool mbar_wait_warp(unsigned long long *bar, unsigned parity) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity);
+  return __shfl_sync(PK_FULL_MASK, ok, 0) != 0;
+}
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -401,8 +408,7 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const float sw = n < a.N ? __ldg(a.w_scales + n) : 0.0f;
       const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
       float sa = SPLIT ? 0.0f : token_scale<C::CH>(a, m0 + half * C::CW);
-      // the outcome is made warp-uniform: tcgen05.ld needs every lane
-      if (!__all_sync(PK_FULL_MASK, mbar_wait(acc_full + buf, (gt >> 1) & 1))) {
+      if (!mbar_wait_warp(acc_full + buf, (gt >> 1) & 1)) {
         if (lane == 0) atomicAdd(&g_wait_timeouts, 1u);
         s_abort = 1;
         break;
@@ -421,13 +427,16 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         } else {
           const int m = m0 + half * C::CW + c;
           const float now = sa;
-          if (c + C::CH < C::CW) sa = token_scale<C::CH>(a, m + C::CH);
+          if (c + C::CH < C::CW) {
+            sa = token_scale<C::CH>(a, m + C::CH);
+          } else {   // the sums are in registers: the accumulator may be filled again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + buf);
+          }
           if (m < a.M) finish_any<E4M3, C::CH>(a, m, n, sw, bias, now, r);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + buf);
     }
   }
   if constexpr (SPLIT) {
@@ -488,22 +497,27 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // instructions per output besides the activation, against 26 for one store per
 // output and token. C must suit TMA (16-byte aligned rows).
 
-#ifndef PEPI
-#define PEPI 8
-#endif
-constexpr int PAIR_EPI = PEPI;
-constexpr int PAIR_THREADS = 32 * (2 + PAIR_EPI);
+constexpr int CN = 16;      // columns finished at a time
+constexpr int BOX_B = 64;   // bytes of a row of a warp's box
+
+// EPI epilogue warps: 16 (four per scheduler) where there is no residual, 8
+// where there is one. With 8 a tile's epilogue takes longer than the products
+// of K = 1024; the residual's rows, read by 16 warps at once, cost more than
+// that gains (12000 x 1024 x 4096 bf16, Swish: 16 warps 62 us, 8 warps 78; 12000
+// x 4096 x 1024 fp32 + residual: 63 and 55).
+template <int EPI>
 struct PairCfg {
+  static constexpr int THREADS = 32 * (2 + EPI);
   static constexpr int BN = 256;
   static constexpr int A_TILE = 128 * BK, B_TILE = BN / 2 * BK;
   static constexpr int STAGE = A_TILE + B_TILE;
-  static constexpr int OUT = PAIR_EPI * 4096;       // a 32-row x 128-byte box per epilogue warp
+  static constexpr int OUT = EPI * 32 * BOX_B;   // a 32-row box per epilogue warp
   static constexpr int PAR = BN * 8;                 // scale and bias of the tile's outputs
   static constexpr int REST = OUT + PAR + 256;
   static constexpr int STAGES = (227 * 1024 - REST) / STAGE < 8 ? (227 * 1024 - REST) / STAGE : 8;
   static constexpr int SMEM = STAGES * STAGE + REST;
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int CW = BN / (PAIR_EPI / 4);   // columns per epilogue warp
+  static constexpr int CW = BN / (EPI / 4);   // columns per epilogue warp
 };
 
 __device__ __forceinline__ unsigned mapa(unsigned saddr, unsigned rank) {
@@ -550,7 +564,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // TMEM columns without waiting; tmem_wait() before the first use.
-__device__ __forceinline__ void tmem_ld32_async(unsigned taddr, unsigned (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_async(unsigned taddr, unsigned (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
       "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
@@ -559,6 +573,13 @@ __device__ __forceinline__ void tmem_ld32_async(unsigned taddr, unsigned (&r)[32
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_async(unsigned taddr, unsigned (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 // The registers pass through, so that no use moves above the wait.
@@ -573,20 +594,27 @@ __device__ __forceinline__ void tmem_wait(unsigned (&r)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_wait(unsigned (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 // 32 entries n .. n + 31 of a row of R as raw 16-byte words (r NULL: none).
 template <typename T>
 struct RowChunk {
   static constexpr int VEC = 16 / (int)sizeof(T);
-  float4 raw[32 / VEC];
+  float4 raw[CN / VEC];
   __device__ __forceinline__ void load(const Args &a, const T *r, int n) {
     if (!r) return;
-    if (a.r_vec && n + 32 <= a.N) {
+    if (a.r_vec && n + CN <= a.N) {
 #pragma unroll
-      for (int i = 0; i < 32 / VEC; i++) raw[i] = *reinterpret_cast<const float4 *>(r + n + i * VEC);
+      for (int i = 0; i < CN / VEC; i++) raw[i] = *reinterpret_cast<const float4 *>(r + n + i * VEC);
     } else {
       T *e = reinterpret_cast<T *>(raw);
 #pragma unroll
-      for (int j = 0; j < 32; j++) e[j] = n + j < a.N ? r[n + j] : from_f32<T>(0.0f);
+      for (int j = 0; j < CN; j++) e[j] = n + j < a.N ? r[n + j] : from_f32<T>(0.0f);
     }
   }
 };
@@ -595,9 +623,9 @@ struct RowChunk {
 // outputs the two scales and the two biases, in shared memory, the same for
 // every lane.
 template <bool E4M3>
-__device__ __forceinline__ void scale_row(const float4 *par, float sa, const unsigned (&acc)[32], float (&v)[32]) {
+__device__ __forceinline__ void scale_row(const float4 *par, float sa, const unsigned (&acc)[CN], float (&v)[CN]) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
+  for (int j = 0; j < CN; j += 2) {
     const float4 p = par[j / 2];
     const float2 s = mul2(make_float2(sum_as_float<E4M3>(acc[j]), sum_as_float<E4M3>(acc[j + 1])), splat2(sa));
     const float2 o = fma2(s, make_float2(p.x, p.y), make_float2(p.z, p.w));
@@ -606,45 +634,47 @@ __device__ __forceinline__ void scale_row(const float4 *par, float sa, const uns
   }
 }
 template <typename T>
-__device__ __forceinline__ void add_residual_row(const Args &a, bool resid, const RowChunk<T> &rc, float (&v)[32]) {
+__device__ __forceinline__ void add_residual_row(const Args &a, bool resid, const RowChunk<T> &rc, float (&v)[CN]) {
   if (resid) {
     const T *x = reinterpret_cast<const T *>(rc.raw);
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = fmaf(v[j], a.rscale, to_f32(x[j]));
+    for (int j = 0; j < CN; j++) v[j] = fmaf(v[j], a.rscale, to_f32(x[j]));
   } else if (a.rscale != 1.0f) {
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] *= a.rscale;
+    for (int j = 0; j < CN; j++) v[j] *= a.rscale;
   }
 }
 
-// 32 finished outputs as chunks 16 bytes wide of this lane's row of the box.
+// CN finished outputs as chunks 16 bytes wide of this lane's row of the box.
+// Chunk c of row r lies at c ^ (r / 2 mod 4): eight rows' chunks fill the banks.
 template <typename T>
-__device__ __forceinline__ void box_row(unsigned char *box, int first, const float (&v)[32]) {
+__device__ __forceinline__ void box_row(unsigned char *box, int first, const float (&v)[CN]) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int j = 0; j < 32; j += VEC) {
+  for (int j = 0; j < CN; j += VEC) {
     alignas(16) T o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) o[i] = from_f32<T>(v[j + i]);
-    const int chunk = (first + j) / VEC;   // chunk c of row r lies at c ^ (r mod 8): no bank conflicts
-    *reinterpret_cast<uint4 *>(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(o);
+    const int chunk = (first + j) / VEC;
+    *reinterpret_cast<uint4 *>(box + lane * BOX_B + ((chunk ^ ((lane >> 1) & 3)) << 4)) =
+        *reinterpret_cast<const uint4 *>(o);
   }
 }
 
-// The box (32 tokens from m0, 128 bytes of outputs from n0) to C: a store of the
-// warp covers four rows, 128 bytes of each.
+// The box (32 tokens from m0, 64 bytes of outputs from n0) to C: a store of the
+// warp covers eight rows, 64 bytes of each.
 template <typename T>
 __device__ __forceinline__ void box_store(const Args &a, const unsigned char *box, int m0, int n0) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  const int lane = threadIdx.x & 31, chunk = lane & 7;
+  const int lane = threadIdx.x & 31, chunk = lane & 3;
   const int n = n0 + chunk * VEC;
-  T *c = static_cast<T *>(a.C) + (long long)(m0 + (lane >> 3)) * a.ldc + n;
+  T *c = static_cast<T *>(a.C) + (long long)(m0 + (lane >> 2)) * a.ldc + n;
   const bool whole = a.c_vec && n + VEC <= a.N;
 #pragma unroll
-  for (int i = 0; i < 8; i++, c += 4 * a.ldc) {
-    const int row = 4 * i + (lane >> 3);
-    const uint4 d = *reinterpret_cast<const uint4 *>(box + row * 128 + ((chunk ^ (row & 7)) << 4));
+  for (int i = 0; i < 4; i++, c += 8 * a.ldc) {
+    const int row = 8 * i + (lane >> 2);
+    const uint4 d = *reinterpret_cast<const uint4 *>(box + row * BOX_B + ((chunk ^ ((row >> 1) & 3)) << 4));
     if (m0 + row < a.M) {
       if (whole) {
         *reinterpret_cast<uint4 *>(c) = d;
@@ -658,10 +688,10 @@ __device__ __forceinline__ void box_store(const Args &a, const unsigned char *bo
   }
 }
 
-template <bool E4M3, typename T>
-__global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
+template <bool E4M3, typename T, int EPI>
+__global__ void __launch_bounds__(PairCfg<EPI>::THREADS, 1) __cluster_dims__(2, 1, 1)
 q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, Args a) {
-  using C = PairCfg;
+  using C = PairCfg<EPI>;
   constexpr int BN = C::BN;
   // the same offsets in both CTAs: an MMA's descriptors serve both
   extern __shared__ __align__(1024) unsigned char pair_smem[];
@@ -691,7 +721,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(acc_full + b, 1);
-      mbar_init(acc_empty + b, 2 * PAIR_EPI);
+      mbar_init(acc_empty + b, 2 * EPI);
     }
     mbar_init(done, 1);
     mbar_init_fence();
@@ -775,19 +805,19 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       mbar_wait(done, 0);
     }
   } else {
-    // warp w: tokens 32 (w % 4) .. + 31 of this CTA's 128, half of the columns
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const unsigned lane_addr = ((unsigned)(q * 32) << 16) + half * C::CW;
-    unsigned char *box = out + (warp - 2) * 4096;
-    float *my_par = par + half * C::CW * 2;   // shared by the four warps of this half
-    constexpr int COLS = 128 / (int)sizeof(T);   // outputs per box
+    // warp w: tokens 32 (w % 4) .. + 31 of this CTA's 128, C::CW of the columns
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    const unsigned lane_addr = ((unsigned)(q * 32) << 16) + part * C::CW;
+    unsigned char *box = out + (warp - 2) * (32 * BOX_B);
+    float *my_par = par + part * C::CW * 2;   // shared by the four warps of this part
+    constexpr int COLS = BOX_B / (int)sizeof(T);   // outputs per box
     int gt = 0;
     bool ok = true;   // after a wait that ran out a warp only keeps the others' barriers going
     for (long long tile = blockIdx.x >> 1; tile < n_tiles; tile += step, gt++) {
       const int m0 = (int)(tile % tiles_m) * 256 + (int)rank * 128 + q * 32;
-      const int n0 = (int)(tile / tiles_m) * BN + half * C::CW;
+      const int n0 = (int)(tile / tiles_m) * BN + part * C::CW;
       const int m = m0 + lane, buf = gt & 1;
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");   // the last tile's pairs are read
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");   // the last tile's pairs are read
       for (int i = q * 32 + lane; i < C::CW; i += 128) {
         const int n = n0 + i, at = (i & ~1) * 2 + (i & 1);
         my_par[at] = n < a.N ? __ldg(a.w_scales + n) : 0.0f;
@@ -797,8 +827,8 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const T *r = a.R && m < a.M ? static_cast<const T *>(a.R) + (long long)m * a.ldr : nullptr;
       RowChunk<T> rc;
       rc.load(a, n0 < a.N ? r : nullptr, n0);
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-      if (ok && !__all_sync(PK_FULL_MASK, mbar_wait(acc_full + buf, (gt >> 1) & 1))) {
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
+      if (ok && !mbar_wait_warp(acc_full + buf, (gt >> 1) & 1)) {
         if (lane == 0) atomicAdd(&g_wait_timeouts, 1u);
         s_abort = 1;
         ok = false;
@@ -807,28 +837,28 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       tc_fence_after();
       // 32 columns at a time; the next ones' TMEM load is in flight while the
       // activation and the store of these go on, and their residual after it
-      unsigned acc[32];
+      unsigned acc[CN];
       const unsigned t0 = tmem + lane_addr + buf * BN;
-      tmem_ld32_async(t0, acc);
+      tmem_ld_async(t0, acc);
       const float4 *p4 = reinterpret_cast<const float4 *>(my_par);
 #pragma unroll 1
-      for (int c = 0; c < C::CW; c += 32) {
-        float v[32];
+      for (int c = 0; c < C::CW; c += CN) {
+        float v[CN];
         tmem_wait(acc);
         scale_row<E4M3>(p4 + c / 2, sa, acc, v);
-        if (c + 32 < C::CW) {
-          tmem_ld32_async(t0 + c + 32, acc);
+        if (c + CN < C::CW) {
+          tmem_ld_async(t0 + c + CN, acc);
         } else {   // this warp's last sums are in registers: the accumulator may be filled again
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(acc_empty + buf), 0));
         }
-        activate<32>(a.act, v);
+        activate<CN>(a.act, v);
         add_residual_row<T>(a, r != nullptr, rc, v);
-        if (c + 32 < C::CW) rc.load(a, n0 + c + 32 < a.N ? r : nullptr, n0 + c + 32);
+        if (c + CN < C::CW) rc.load(a, n0 + c + CN < a.N ? r : nullptr, n0 + c + CN);
         const int first = c & (COLS - 1);   // this chunk's place in its box
         box_row<T>(box, first, v);
-        if (first + 32 == COLS) {
+        if (first + CN == COLS) {
           __syncwarp();
           if (n0 + c - first < a.N) box_store<T>(a, box, m0, n0 + c - first);
           __syncwarp();
@@ -908,10 +938,15 @@ int tmap_bytes(CUtensorMap *map, const void *base, long long rows, long long col
 }
 
 template <bool E4M3, int BQ, bool SPLIT>
+int *narrow_flags() {
+  static int flags[64];
+  return flags;
+}
+
+template <bool E4M3, int BQ, bool SPLIT>
 int launch(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, int split, cudaStream_t s) {
   using C = q8::Cfg<BQ>;
-  static int flags[64];
-  smem_optin(q8::q8_gemm_kernel<E4M3, BQ, SPLIT>, C::SMEM, flags);
+  smem_optin(q8::q8_gemm_kernel<E4M3, BQ, SPLIT>, C::SMEM, narrow_flags<E4M3, BQ, SPLIT>());
   const long long tiles = (long long)((a.M + BQ - 1) / BQ) * ((a.N + q8::BP - 1) / q8::BP);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(q8::THREADS);
@@ -932,23 +967,30 @@ int launch(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, in
   return pkcu_launch_status("pkcu_wmatmul_q8");
 }
 
-template <bool E4M3, typename T>
+template <bool E4M3, typename T, int EPI>
 int launch_pair(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, cudaStream_t s) {
-  using C = q8::PairCfg;
+  using C = q8::PairCfg<EPI>;
   static int flags[64];
-  smem_optin(q8::q8_pair_kernel<E4M3, T>, C::SMEM, flags);
+  smem_optin(q8::q8_pair_kernel<E4M3, T, EPI>, C::SMEM, flags);
   const long long tiles = (long long)((a.M + 255) / 256) * ((a.N + C::BN - 1) / C::BN);
   const long long pairs = pkcu_sm_count() / 2;
   const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
-  q8::q8_pair_kernel<E4M3, T><<<grid, q8::PAIR_THREADS, C::SMEM, s>>>(W->map, ma, a);
+  q8::q8_pair_kernel<E4M3, T, EPI><<<grid, C::THREADS, C::SMEM, s>>>(W->map, ma, a);
   return pkcu_launch_status("pkcu_wmatmul_q8");
 }
 
+template <bool E4M3, typename T>
+int launch_pair_as(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, cudaStream_t s) {
+  return a.R ? launch_pair<E4M3, T, 8>(W, ma, a, s) : launch_pair<E4M3, T, 16>(W, ma, a, s);
+}
+template <typename T>
+int launch_pair_type(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, cudaStream_t s) {
+  return W->e4m3 ? launch_pair_as<true, T>(W, ma, a, s) : launch_pair_as<false, T>(W, ma, a, s);
+}
 int launch_pair_any(const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::Args &a, cudaStream_t s) {
-  if (a.dtype == PKCU_DTYPE_F32) return W->e4m3 ? launch_pair<true, float>(W, ma, a, s) : launch_pair<false, float>(W, ma, a, s);
-  if (a.dtype == PKCU_DTYPE_BF16)
-    return W->e4m3 ? launch_pair<true, __nv_bfloat16>(W, ma, a, s) : launch_pair<false, __nv_bfloat16>(W, ma, a, s);
-  return W->e4m3 ? launch_pair<true, __half>(W, ma, a, s) : launch_pair<false, __half>(W, ma, a, s);
+  if (a.dtype == PKCU_DTYPE_F32) return launch_pair_type<float>(W, ma, a, s);
+  if (a.dtype == PKCU_DTYPE_BF16) return launch_pair_type<__nv_bfloat16>(W, ma, a, s);
+  return launch_pair_type<__half>(W, ma, a, s);
 }
 
 template <bool E4M3, bool SPLIT>
@@ -961,29 +1003,64 @@ int launch_bq(int bq, const pkcu_weight_q8 *W, const CUtensorMap &ma, const q8::
   }
 }
 
+// Clusters of `split` CTAs of the narrow kernel that run at the same time on the
+// current device (one CTA per SM; a cluster lies within a GPC, so fewer than
+// SMs / split). Asked of the runtime once per device.
+int cluster_slots(int split) {
+  static int slots[64][4];
+  const int dev = pkcu_device(), k = split == 2 ? 1 : split == 4 ? 2 : 3;
+  int n = dev < 64 ? __atomic_load_n(&slots[dev][k], __ATOMIC_ACQUIRE) : 0;
+  if (n) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pkcu_sm_count() / split * split));
+  cfg.blockDim = dim3(q8::THREADS);
+  cfg.dynamicSmemBytes = q8::Cfg<16>::SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  smem_optin(q8::q8_gemm_kernel<false, 16, true>, q8::Cfg<16>::SMEM, narrow_flags<false, 16, true>());
+  if (cudaOccupancyMaxActiveClusters(&n, q8::q8_gemm_kernel<false, 16, true>, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = pkcu_sm_count() / split / 2 + 1;
+  }
+  if (dev < 64) __atomic_store_n(&slots[dev][k], n, __ATOMIC_RELEASE);
+  return n;
+}
+
 constexpr int PAIR = 256;   // the pair kernel's tokens per tile
 struct Plan {
   int bq, split;
 };
-// DISPATCH-COMMENT
-Plan plan(int M, int N, int nkb, int sms) {
-  const char *e1 = getenv("BQ"), *e2 = getenv("SMAX");
-  if (e1) {
-    Plan p = {atoi(e1), e2 ? atoi(e2) : 1};
-    return p;
-  }
-  static const float fixed_us[5] = {3.3f, 4.0f, 5.0f, 7.0f, 8.9f};
+// Tile (tokens: 16 .. 128 of the one-CTA kernel, 256 of the pair kernel) and split
+// of K with the least modelled time: a set-up, the first tile's products, then
+// per further tile of a CTA the longer of its products and its epilogue, and the
+// last epilogue. Measured on a B200: 0.34 us per 128 of K for any tile of one
+// CTA or pair, the epilogues below (the pair kernel's stores of one entry at a
+// time where rows of C are not 16-byte aligned), about 2 us for a cluster's
+// launch and exchange. Over 14 token counts (1 .. 2000) x 4 weights the choice was
+// within 5 % of the best tile and split: M = 128, 1024 -> 4096: 16 tokens 9.1 us, 32
+// 6.7, 64 7.3, 128 8.6, pair 12.2; M = 375, 4096 -> 1024: 128 tokens alone 17.7, split
+// in two 17.1, in four 12.5, pair 23.9.
+Plan plan(int M, int N, int nkb, bool c_vec) {
+  static const float epi_us[5] = {0.8f, 1.25f, 2.0f, 3.3f, 5.5f};
+  const int sms = pkcu_sm_count();
   Plan best = {PAIR, 1};
   float best_us = INFINITY;
-  const long long tiles_n = ((long long)N + q8::BP - 1) / q8::BP;
   for (int i = 0; i < 5; i++) {
     const int bq = 16 << i;
     const bool pair = bq == PAIR;
-    const long long tiles = ((long long)M + bq - 1) / bq * (pair ? ((long long)N + 255) / 256 : tiles_n);
-    const long long slots = pair ? sms / 2 : sms;
-    for (int split = 1; split <= (pair ? 1 : 8) && split <= nkb && (split == 1 || tiles * split <= sms); split *= 2) {
-      const float waves = (float)((tiles * split + slots - 1) / slots);
-      const float us = fixed_us[i] + (split > 1 ? 2.0f + 0.2f * split : 0.0f) + waves * (float)((nkb + split - 1) / split) * 0.34f;
+    const int bn = pair ? 256 : q8::BP;
+    const long long tiles = (((long long)M + bq - 1) / bq) * (((long long)N + bn - 1) / bn);
+    const float epi = pair && !c_vec ? 14.0f : epi_us[i];
+    for (int split = 1; split <= (pair ? 1 : 8) && split <= nkb; split *= 2) {
+      if (split > 1 && (tiles * split > sms || tiles > cluster_slots(split))) break;
+      const long long slots = pair ? sms / 2 : sms;
+      const float products = (float)((nkb + split - 1) / split) * 0.34f;
+      const float more = split > 1 ? 0.0f : (float)((tiles + slots - 1) / slots - 1);
+      const float us = 2.7f + products + more * (products > epi ? products : epi) + epi + (split > 1 ? 2.0f + 0.2f * split : 0.0f);
       if (us < best_us) {
         best_us = us;
         best.bq = bq;
@@ -993,7 +1070,6 @@ Plan plan(int M, int N, int nkb, int sms) {
   }
   return best;
 }
-
 }  // namespace
 
 extern "C" int pk_q8_wait_timeouts(unsigned *count, int reset) { return q8::pk_q8_wait_timeouts_acc(count, reset); }
@@ -1096,7 +1172,7 @@ extern "C" int pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scal
   a.nkb = (W->K + q8::BK - 1) / q8::BK;
   a.r_vec = PK_ALIGNED16(R) && ldr * size % 16 == 0;
   a.c_vec = PK_ALIGNED16(C) && ldc * size % 16 == 0;
-  const Plan p = plan(M, W->N, a.nkb, pkcu_sm_count());
+  const Plan p = plan(M, W->N, a.nkb, a.c_vec != 0);
   CUtensorMap ma;
   const int st = tmap_bytes(&ma, A, M, W->K, lda, p.bq == PAIR ? 128 : p.bq);
   if (st) return st;
