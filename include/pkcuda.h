@@ -331,6 +331,28 @@ int  pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scales, const 
                      const float *bias, int act, const void *R, long long ldr, float rscale,
                      void *C, long long ldc, int dtype, int M, pkcu_stream_t stream);
 
+/* One token per row of logits [n_rows, ld], V of each row used (type F32, BF16
+ * or F16; V up to 262144), drawn with given numbers. Per row (arrays [n_rows],
+ * each may be NULL):
+ *   temperature T  weights w = exp((l - max l) / T); NULL: 1. T <= 0 or NaN:
+ *                  greedy, the first largest, log-probability 0
+ *   top_k          the k largest stay; NULL or k <= 0: all
+ *   top_p          of these the fewest largest whose weights sum to at least
+ *                  top_p times all of them (one at least); NULL, >= 1 or NaN: all
+ *   min_p          of these what has w >= min(min_p, 1); NULL, <= 0 or NaN: all
+ * Among equal logits the lower index is the larger (+0 and -0 are equal).
+ * tokens[r] is the first index at which the running sum of the kept weights, in
+ * index order, exceeds u[r] times their total (u in [0, 1); below 0 or NaN: 0,
+ * from 1 on: the last kept). logprobs[r] (the array may be NULL): log of the
+ * token's weight over that total. Logits of -infinity and NaN are never taken;
+ * a row with nothing else gives token -1 and log-probability -infinity. Weights
+ * are held to 2^-44 of the largest and summed exactly: the result does not
+ * depend on the order of any sum, and what weighs less is never drawn. */
+int pkcu_sample_rows(const void *logits, int dtype, long long ld, const float *temperature,
+                     const int32_t *top_k, const float *top_p, const float *min_p,
+                     const float *u, int32_t *tokens, float *logprobs, long long n_rows, int V,
+                     pkcu_stream_t stream);
+
 /* ── 3. sequence driver ──────────────────────────────────────────────────── */
 
 /* Non-GEMM parameters of one conformer block (csrc/parakeet.h:78-125). */

@@ -68,6 +68,7 @@ EXPORTED = (
     "pkcu_encoder_nongemm_fused", "pkcu_conv_weight_create", "pkcu_pointwise_conv1d",
     "pkcu_pointwise_conv1d_glu", "pkcu_residual_rms_norm_q8",
     "pkcu_weight_q8_create", "pkcu_weight_q8_destroy", "pkcu_wmatmul_q8",
+    "pkcu_sample_rows",
 )
 
 
@@ -203,6 +204,7 @@ _SIGS = {
     "pkcu_conv_weight_create": (I, [VP, I, I, I, VP, C.POINTER(VP)]),
     "pkcu_pointwise_conv1d": (I, [VP, VP, VP, VP, I, VP, VP]),
     "pkcu_pointwise_conv1d_glu": (I, [VP, VP, VP, VP, I, VP, VP]),
+    "pkcu_sample_rows": (I, [VP, I, LL, VP, VP, VP, VP, VP, VP, VP, LL, I, VP]),
     "pkcu_weight_q8_create": (I, [VP, I, VP, I, I, I, VP, C.POINTER(VP)]),
     "pkcu_weight_q8_destroy": (None, [VP]),
     "pkcu_wmatmul_q8": (I, [VP, LL, VP, VP, VP, I, VP, LL, F, VP, LL, I, I, VP]),
@@ -401,6 +403,26 @@ def wmatmul_q8(a, a_scales, weight, out, bias=None, act=None, residual=None, rsc
     ldr = 0 if residual is None else residual.stride(0) if M > 1 else max(residual.stride(0), weight.N)
     _call_on(a, stream, "pkcu_wmatmul_q8", a.data_ptr(), lda, a_scales.data_ptr(), weight.handle, ptr(bias),
              _ACTS[act], ptr(residual), ldr, rscale, out.data_ptr(), ldc, dtype_of(out), M)
+
+
+def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                stream=None) -> None:
+    """pkcu_sample_rows on tensors: logits [n_rows, V] with packed columns,
+    tokens int32 [n_rows]; temperature, top_p, min_p, u, logprobs fp32 and top_k
+    int32 [n_rows] (all but u may be None)."""
+    import torch
+    _require(logits.dim() == 2 and logits.is_cuda and (logits.stride(1) == 1 or logits.shape[1] == 1),
+             "logits: [n_rows, V] on the GPU with packed columns is needed")
+    rows, V = logits.shape
+    for t in (tokens, top_k):
+        _require(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == rows),
+                 "tokens and top_k: packed int32 tensors of one entry per row are needed")
+    for t, what in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (logprobs, "logprobs")):
+        _vector(t, rows, what)
+    _same_device(logits, u, tokens, logprobs, temperature, top_k, top_p, min_p)
+    _call_on(logits, stream, "pkcu_sample_rows", logits.data_ptr(), dtype_of(logits),
+             logits.stride(0) if rows > 1 else max(logits.stride(0), V), ptr(temperature), ptr(top_k), ptr(top_p),
+             ptr(min_p), u.data_ptr(), tokens.data_ptr(), ptr(logprobs), rows, V)
 
 
 class Seq:

@@ -53,3 +53,22 @@ def test_weight_q8_refusals(L, change, word):
 def test_product_needs_a_weight(L):
     assert L.pkcu_wmatmul_q8(P, 64, P, None, None, 2, None, 0, 1.0, P, 64, 0, 4, None) == ERR_ARG
     assert b"NULL weight" in L.pkcu_last_error()
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(n_rows=-1), "rows"), (dict(V=0), "rows"), (dict(V=262145), "rows"), (dict(dtype=1), "type"),
+    (dict(dtype=5), "type"), (dict(logits=None), "NULL"), (dict(u=None), "NULL"), (dict(tokens=None), "NULL"),
+    (dict(ld=1024), "ld"), (dict(logits=P + 2), "aligned"), (dict(top_k=P + 1), "aligned"),
+    (dict(logprobs=P + 2), "aligned")])
+def test_sample_refusals(L, change, word):
+    a = dict(logits=P, dtype=0, ld=1025, temperature=None, top_k=P, top_p=P, min_p=None, u=P, tokens=P, logprobs=P,
+             n_rows=3, V=1025)
+    a.update(change)
+    assert L.pkcu_sample_rows(*a.values(), None) == ERR_ARG
+    msg = L.pkcu_last_error().decode()
+    assert "pkcu_sample_rows" in msg and word in msg, msg
+
+
+def test_no_rows(L):
+    assert L.pkcu_sample_rows(None, 0, 10, None, None, None, None, None, None, None, 0, 10, None) == 0
+    assert L.pkcu_residual_rms_norm_q8(None, None, None, 1.0, None, 1e-5, 0, None, None, 1, 10, None, 0, 10, None) == 0
