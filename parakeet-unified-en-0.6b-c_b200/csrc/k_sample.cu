@@ -47,7 +47,7 @@ namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
 constexpr int MAX_V = 1 << 18;            // sums of weights <= 2^44 fit 62 bits
-constexpr int SMEM_LOGITS = 128 * 1024;   // bytes of logits a CTA holds at most
+constexpr int SMEM_VALUES = 128 * 1024;     // bytes of values a CTA holds at most
 enum { WARP, CTA, CLUSTER };              // what a row's group is
 
 struct Args {
@@ -60,15 +60,16 @@ struct Args {
   float *logprobs;
 };
 
-// Entries as unsigned keys in the order of the values, 0 for what is never
-// taken (-infinity, NaN); -0 counts as 0.
+// Entries in shared memory are fp32 values, -infinity for what is never taken
+// (-infinity, NaN), +0 for zeros of both signs. Keys: finite and +infinite values
+// as unsigned numbers in the same order, for halving a range of values.
+__device__ __forceinline__ float clean(float v) { return __fadd_rn(fmaxf(v, -INFINITY), 0.0f); }
 __device__ __forceinline__ unsigned key_of(float v) {
-  if (!(v > -INFINITY)) return 0;
-  const unsigned b = __float_as_uint(__fadd_rn(v, 0.0f));
-  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  const unsigned b = __float_as_uint(v);
+  return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float value_of(unsigned key) {
-  return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+__device__ __forceinline__ float value_of(unsigned k) {
+  return __uint_as_float(k ^ (~(unsigned)((int)k >> 31) | 0x80000000u));
 }
 
 // 2^(i / 16)
@@ -77,35 +78,39 @@ __constant__ double kPow2[16] = {
     1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407,
     1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 
-// exp((v - max) / T) as an integer multiple of 2^-44, rounded; exactly 2^44 for
-// v = max. With y = (v - max) 16 log2(e) / T = n + r, |r| <= 1/2: 2^(y / 16) =
+// exp((v - max) / T) as an integer multiple of 2^-44, rounded; 2^44 for v = max
+// (finite). With y = (v - max) 16 log2(e) / T = n + r, |r| <= 1/2: 2^(y / 16) =
 // 2^(n div 16) 2^((n mod 16) / 16) e^(r ln 2 / 16), the last by the Taylor series
 // of degree 5 (|r ln 2 / 16| < 0.0217: the next term is below 1.5e-13). Sums that
-// round to an integer are formed by adding 1.5 2^52.
+// round to an integer are formed by adding 1.5 2^52. Below `least`, where the
+// weight is under 2^-60, the result is 0 whatever the arithmetic gives.
 struct Weight {
   const double *tab;   // kPow2 in shared memory
-  double c;            // 16 log2(e) / T
-  float max;
+  double c, top;       // 16 log2(e) / T; max
+  float max, least;
+  __device__ __forceinline__ void set(float m, float temp) {
+    max = m;
+    top = (double)m;
+    c = 16.0 * 1.44269504088896340736 / (double)temp;
+    least = __fsub_rn(m, __fmul_rn(41.6f, temp));   // 60 ln 2 = 41.59; rounds to a float no entry lies between
+  }
   __device__ __forceinline__ u64 operator()(float v) const {
-    if (v == max) return 1ull << 44;
-    // the maximum of a difference and a limit: also NaN (infinite max, T) becomes the limit
-    const double d = (double)v - (double)max;
-    const double y = fmax(__dmul_rn(d, c), -16.0 * 60.0);
+    const double d = __dadd_rn((double)v, -top);
     constexpr double kShift = 6755399441055744.0;   // 1.5 2^52
-    const double t = __dadd_rn(y, kShift);
-    const double r = __dadd_rn(y, -__dadd_rn(t, -kShift));
+    const double t = fma(d, c, kShift);
+    const double r = fma(d, c, -__dadd_rn(t, -kShift));
     const int n = __double2loint(t);
     constexpr double L = 0.693147180559945309417 / 16;
-    const double z = r * L;
-    double p = fma(z, 1.0 / 120, 1.0 / 24);
-    p = fma(z, p, 1.0 / 6);
-    p = fma(z, p, 0.5);
-    p = fma(z, p, 1.0);
-    p = fma(z, p, 1.0);
+    const double r2 = __dmul_rn(r, r);
+    double p = fma(fma(r, L * L * L * L * L / 120, L * L * L * L / 24), r2, fma(r, L * L * L / 6, L * L / 2));
+    p = fma(p, r2, fma(r, L, 1.0));
     const double w = __dmul_rn(tab[n & 15], p);
     // times 2^(n div 16 + 44), then to an integer
     const double s = __hiloint2double(__double2hiint(w) + (((n >> 4) + 44) << 20), __double2loint(w));
-    return (u64)__double_as_longlong(__dadd_rn(s, 4503599627370496.0)) & 0xfffffffffffffull;   // + 2^52
+    const double q = __dadd_rn(s, 4503599627370496.0);   // + 2^52
+    const bool in = v >= least;
+    const unsigned hi = in ? (unsigned)__double2hiint(q) & 0xfffffu : 0, lo = in ? (unsigned)__double2loint(q) : 0;
+    return (u64)hi << 32 | lo;
   }
 };
 
@@ -113,34 +118,35 @@ struct Weight {
 template <int MODE>
 struct Shared {
   static constexpr int NB = MODE == WARP ? 256 : 1024;    // bins
-  static constexpr int CAP = MODE == WARP ? 128 : 1024;   // entries of the list
+  static constexpr int CAP = MODE == WARP ? 256 : 2048;   // entries of the list
   static constexpr int RANK = MODE == WARP ? 64 : 512;    // candidates ranked against each other
   static constexpr int NW = MODE == WARP ? 1 : 32;
   u64 part_w[2][NW];        // a warp's part of a reduction or scan; alternating
-  unsigned part_n[2][NW], part_lo[2][NW], part_hi[2][NW];
+  unsigned part_n[2][NW];
+  float part_lo[2][NW], part_hi[2][NW];
   u64 cta_w[2];             // this CTA's part, read by the cluster; alternating
-  unsigned cta_n[2], cta_lo[2], cta_hi[2];
+  unsigned cta_n[2];
+  float cta_lo[2], cta_hi[2];
   u64 all_w[RANK];
   float all[RANK];
   float cand[RANK];         // this CTA's candidates, read by the cluster
-  union {
-    unsigned cnt[NB];
-    float mass[NB];
-  };
+  unsigned bins[NB];        // counts, or weights in hint units
   float list[CAP];          // this CTA's list: values and indices, in index order
   int index[CAP];
   unsigned n_cand;
   int bin;
-  unsigned cut_key, cut_take, cut_ties;
+  unsigned bin_before, bin_inside;
+  float cut;
+  unsigned cut_take, cut_ties;
 };
 
 // Sums and extremes over a row's entries.
 struct Sums {
-  u64 w;            // weights
-  unsigned n;       // entries
-  unsigned lo, hi;  // smallest, largest key
+  u64 w;         // weights
+  unsigned n;    // entries
+  float lo, hi;  // smallest, largest value
 };
-__device__ __forceinline__ Sums no_sums() { return Sums{0, 0, 0xffffffffu, 0}; }
+__device__ __forceinline__ Sums no_sums() { return Sums{0, 0, INFINITY, -INFINITY}; }
 
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 #pragma unroll
@@ -158,11 +164,10 @@ __device__ __forceinline__ u64 warp_scan_u64(u64 v) {   // inclusive
 }
 
 // Where entries come from: the row in shared memory, or the list.
-template <typename T>
 struct FromRow {
-  const T *x;
+  const float *x;
   int n, base;
-  __device__ __forceinline__ float value(int i) const { return to_f32(x[i]); }
+  __device__ __forceinline__ float value(int i) const { return x[i]; }
   __device__ __forceinline__ int index(int i) const { return base + i; }
 };
 struct FromList {
@@ -178,15 +183,17 @@ struct Row {
   typedef Shared<MODE> S;
   const Args &a;
   S &s;
-  T *x;                 // this group's (CTA's) entries
+  float *x;             // this group's (CTA's) entries
   int base, n;          // the first one's index in the row, their number
   unsigned rank, size;  // of the cluster
-  int tid, nt;          // thread of the group (CTA), threads
+  int tid;              // thread of the group (CTA)
   int flip, cflip;
   Weight weight;
-  float max, scale;     // bins: (max - l) scale
+  float scale;          // bins: (max - l) scale
+  int hint;             // bins of weights: units of 2^(hint - 44)
 
   // ── the group ──
+  __device__ __forceinline__ int nt() const { return MODE == WARP ? 32 : (int)blockDim.x; }
   __device__ __forceinline__ void lsync() const {   // this group's (CTA's) threads
     if (MODE == WARP) __syncwarp();
     else __syncthreads();
@@ -201,7 +208,7 @@ struct Row {
   }
 
   // Totals over the row's threads, to every thread. What is asked for: W weights,
-  // N entries, K extreme keys.
+  // N entries, K extreme values.
   template <bool W, bool N, bool K>
   __device__ __forceinline__ Sums total(Sums v) {
     const int lane = threadIdx.x & 31;
@@ -258,8 +265,11 @@ struct Row {
     if (W) v.w = warp_sum_u64(v.w);
     if (N) v.n = __reduce_add_sync(PK_FULL_MASK, v.n);
     if (K) {
-      v.lo = __reduce_min_sync(PK_FULL_MASK, v.lo);
-      v.hi = __reduce_max_sync(PK_FULL_MASK, v.hi);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        v.lo = fminf(v.lo, __shfl_xor_sync(PK_FULL_MASK, v.lo, o));
+        v.hi = fmaxf(v.hi, __shfl_xor_sync(PK_FULL_MASK, v.hi, o));
+      }
     }
   }
 
@@ -301,100 +311,103 @@ struct Row {
   }
 
   // ── bins ──
-  // Linear in max - l, the last bin open-ended (and for an infinite maximum's NaN).
-  __device__ __forceinline__ int bin_of(unsigned k) const {
-    const float f = (max - value_of(k)) * scale;
-    return f < (float)(S::NB - 1) ? (int)f : S::NB - 1;
+  // Linear in max - l, rounded, the last one open-ended.
+  __device__ __forceinline__ int bin_of(float v) const {
+    const float f = __fmul_rn(__fsub_rn(weight.max, v), scale);
+    return __float_as_int(__fadd_rn(fminf(f, (float)(S::NB - 1)), 8388608.0f)) - 0x4B000000;
+  }
+  // A value that every entry of the bins up to `bin` is at least (a few of the next
+  // bin's may be too): the bin's lower edge, a tenth of a bin further down. The
+  // margin covers the roundings of bin_of (2 x 2^-24 of at most 1023 bins); the
+  // edge's own rounding to a float passes no entry, as those are floats as well.
+  __device__ __forceinline__ float edge_of(int bin) const {
+    return bin >= S::NB - 1 ? -INFINITY : __fsub_rn(weight.max, __fdiv_rn((float)bin + 0.6f, scale));
   }
   __device__ __forceinline__ void clear_bins() {
     lsync();
-    for (int b = tid; b < S::NB; b += nt) s.cnt[b] = 0;
+    for (int b = tid; b < S::NB; b += nt()) s.bins[b] = 0;
     lsync();
   }
-  // The first bin at which the bins' running sum reaches target, `before` what the
-  // bins before it hold and `inside` what it holds itself (BY_WEIGHT: a hint, in fp32).
-  template <bool BY_WEIGHT>
-  __device__ int find_bin(u64 target, unsigned &before, unsigned &inside) {
+  // The first bin at which the bins' running sum reaches goal, `before` what the
+  // bins before it hold, `inside` what it holds itself, `all` what all hold.
+  __device__ int find_bin(u64 goal, unsigned &before, unsigned &inside, u64 &all) {
     gsync();   // every CTA's bins are filled
-    const int per = (S::NB + nt - 1) / nt, b0 = tid * per;
-    float run_w = 0.0f;
-    unsigned run_n = 0;
-    for (int b = b0; b < b0 + per && b < S::NB; b++)
-      for (unsigned r = 0; r < (MODE == CLUSTER ? size : 1); r++) {
-        if (BY_WEIGHT) run_w += *peer(&s.mass[b], r);
-        else run_n += *peer(&s.cnt[b], r);
+    constexpr int MAXPER = MODE == WARP ? S::NB / 32 : 8;   // at least 128 threads in a CTA
+    const int per = (S::NB + nt() - 1) / nt(), b0 = tid * per;
+    unsigned held[MAXPER];
+    u64 mine = 0;
+#pragma unroll
+    for (int j = 0; j < MAXPER; j++) {
+      held[j] = 0;
+      if (j < per && b0 + j < S::NB) {
+        u64 c = 0;
+        for (unsigned r = 0; r < (MODE == CLUSTER ? size : 1); r++) c += *peer(&s.bins[b0 + j], r);
+        held[j] = (unsigned)c;   // the row's total fits 32 bits
       }
-    // hints in units of 2^-40 of the largest weight, so that one integer scan serves
-    // both (and, being integers, agrees in every CTA of a cluster)
-    const u64 mine = BY_WEIGHT ? (u64)(run_w * 0x1p40f) : run_n;
-    const u64 goal = BY_WEIGHT ? (target >> 4 ? target >> 4 : 1) : target;
-    u64 run;
-    {   // the bins are the row's already: scan this CTA's threads only
-      const u64 inc = warp_scan_u64(mine);
-      run = inc - mine;
-      const u64 all = __shfl_sync(PK_FULL_MASK, inc, 31);
-      if (MODE != WARP) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-        if (lane == 0) s.part_w[flip][warp] = all;
-        if (threadIdx.x == 0) s.bin = S::NB - 1;
-        __syncthreads();
-        const u64 w = warp_scan_u64(lane < nw ? s.part_w[flip][lane] : 0);
-        flip ^= 1;
-        if (warp > 0) run += __shfl_sync(PK_FULL_MASK, w, warp - 1);
-      } else {
-        if (tid == 0) s.bin = S::NB - 1;
-        __syncwarp();
-      }
+      mine += held[j];
     }
+    const u64 inc = warp_scan_u64(mine);
+    u64 run = inc - mine;
+    all = __shfl_sync(PK_FULL_MASK, inc, 31);
+    if (tid == 0) s.bin = S::NB - 1;
+    if (MODE != WARP) {
+      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+      if (lane == 0) s.part_w[flip][warp] = all;
+      __syncthreads();
+      const u64 w = warp_scan_u64(lane < nw ? s.part_w[flip][lane] : 0);
+      flip ^= 1;
+      if (warp > 0) run += __shfl_sync(PK_FULL_MASK, w, warp - 1);
+      all = __shfl_sync(PK_FULL_MASK, w, 31);
+    } else {
+      __syncwarp();
+    }
+    if (goal > all) goal = all;   // hints: roundings may have lost the last
     if (run < goal && goal <= run + mine) {
-      int b = b0;
-      u64 c = 0;
-      for (;; b++) {
-        float bw = 0.0f;
-        unsigned bn = 0;
-        for (unsigned r = 0; r < (MODE == CLUSTER ? size : 1); r++) {
-          if (BY_WEIGHT) bw += *peer(&s.mass[b], r);
-          else bn += *peer(&s.cnt[b], r);
+      int b = -1;
+      u64 at = run;
+#pragma unroll
+      for (int j = 0; j < MAXPER; j++)
+        if (b < 0) {
+          if (at + held[j] >= goal) {
+            b = b0 + j;
+            s.bin_before = (unsigned)at;
+            s.bin_inside = held[j];
+          }
+          at += held[j];
         }
-        c = BY_WEIGHT ? (u64)(bw * 0x1p40f) : bn;
-        if (run + c >= goal || b == b0 + per - 1 || b == S::NB - 1) break;
-        run += c;
-      }
       s.bin = b;
-      s.cut_take = (unsigned)run;
-      s.cut_ties = (unsigned)c;
     }
     lsync();
-    before = s.cut_take;
-    inside = s.cut_ties;
+    before = s.bin_before;
+    inside = s.bin_inside;
     return s.bin;
   }
 
-  // The border of a prefix of the order among a source's entries with key > above:
-  // the first of them, from the largest, at which the count (BY_WEIGHT: the weight)
-  // reaches `target` (1 .. what there is), given the bins of these entries. Leaves
-  // s.cut_key, the border's key, s.cut_take, how many of its equals belong to the
-  // prefix, s.cut_ties, how many there are.
+  // The border of a prefix of the order among a source's entries > above: the first
+  // of them, from the largest, at which the count (BY_WEIGHT: the weight) reaches
+  // `target` (1 .. what there is), given the bin that the bins of these entries
+  // say. Leaves s.cut, the border's value, s.cut_take, how many of its equals
+  // belong to the prefix, s.cut_ties, how many there are.
   template <bool BY_WEIGHT, typename Src>
-  __device__ void border(const Src &src, unsigned above, u64 target, int bin, unsigned bin_before, unsigned bin_inside) {
-    unsigned hi = 0xffffffffu, lo = above;    // the border's key is in (lo, hi]
-    u64 before = bin_before;                  // count or weight of the keys > hi
-    unsigned inside = bin_inside;             // entries with keys in (lo, hi]
-    bool found = !BY_WEIGHT;                  // counts need no confirmation, only the bin's keys
+  __device__ void border(const Src &src, float above, u64 target, int bin, unsigned bin_before, unsigned bin_inside) {
+    float hi = INFINITY, lo = above;          // the border is in (lo, hi], or [lo, hi] once `found`
+    u64 before = bin_before;                  // count or weight of the values > hi
+    unsigned inside = bin_inside;             // entries there
+    bool found = !BY_WEIGHT;                  // counts need no confirmation, only the bin's values
     for (int tries = 0; tries < (BY_WEIGHT ? 3 : 1); tries++) {
       Sums up = no_sums(), in = no_sums();
-      for (int i = tid; i < src.n; i += nt) {
-        const unsigned k = key_of(src.value(i));
-        if (k <= above) continue;
-        const int b = bin_of(k);
+      for (int i = tid; i < src.n; i += nt()) {
+        const float v = src.value(i);
+        if (!(v > above)) continue;
+        const int b = bin_of(v);
         if (b > bin) continue;
-        const u64 w = BY_WEIGHT ? weight(value_of(k)) : 0;
+        const u64 w = BY_WEIGHT ? weight(v) : 0;
         if (b < bin) {
           up.w += w;
         } else {
           in.n++;
-          in.lo = min(in.lo, k);
-          in.hi = ::max(in.hi, k);
+          in.lo = fminf(in.lo, v);
+          in.hi = fmaxf(in.hi, v);
           in.w += w;
         }
       }
@@ -407,38 +420,41 @@ struct Row {
       }
       if (found) {
         hi = in.hi;
-        lo = in.lo - 1;
+        lo = in.lo;
         break;
       }
-      bin = target <= up.w ? ::max(bin - 1, 0) : min(bin + 1, S::NB - 1);   // a rounding of the hint: one bin off
+      bin = target <= up.w ? max(bin - 1, 0) : min(bin + 1, S::NB - 1);   // a rounding of the hint: one bin off
     }
     if (!found) {   // all of them
       Sums in = no_sums();
-      for (int i = tid; i < src.n; i += nt) {
-        const unsigned k = key_of(src.value(i));
-        if (k <= above) continue;
+      for (int i = tid; i < src.n; i += nt()) {
+        const float v = src.value(i);
+        if (!(v > above)) continue;
         in.n++;
-        in.hi = ::max(in.hi, k);
+        in.lo = fminf(in.lo, v);
+        in.hi = fmaxf(in.hi, v);
       }
       in = total<false, true, true>(in);
       inside = in.n;
+      lo = in.lo;
       hi = in.hi;
       before = 0;
     }
-    // too many to rank: halve the range of keys until few are left, or one key
-    while (inside > (unsigned)S::RANK && hi - lo > 1) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      Sums up = no_sums();   // keys in (mid, hi]
-      for (int i = tid; i < src.n; i += nt) {
-        const unsigned k = key_of(src.value(i));
-        if (k <= mid || k > hi) continue;
+    // too many to rank: halve the range of values (as keys) until few are left, or one value
+    while (inside > (unsigned)S::RANK && lo < hi) {
+      const unsigned kl = key_of(lo);
+      const float mid = value_of(kl + (key_of(hi) - kl) / 2);   // lo <= mid < hi
+      Sums up = no_sums();   // values in (mid, hi]
+      for (int i = tid; i < src.n; i += nt()) {
+        const float v = src.value(i);
+        if (!(v > mid) || v > hi) continue;
         up.n++;
-        if (BY_WEIGHT) up.w += weight(value_of(k));
+        if (BY_WEIGHT) up.w += weight(v);
       }
       up = total<BY_WEIGHT, true, false>(up);
       const u64 more = BY_WEIGHT ? up.w : up.n;
       if (before + more >= target) {
-        lo = mid;
+        lo = value_of(key_of(mid) + 1);
         inside = up.n;
       } else {
         before += more;
@@ -449,8 +465,8 @@ struct Row {
     lsync();   // the caller's and the bin search's words are read
     if (inside > (unsigned)S::RANK) {   // all equal
       if (tid == 0) {
-        const u64 each = BY_WEIGHT ? weight(value_of(hi)) : 1;
-        s.cut_key = hi;
+        const u64 each = BY_WEIGHT ? weight(hi) : 1;
+        s.cut = hi;
         s.cut_ties = inside;
         s.cut_take = (unsigned)((target - before + each - 1) / each);
       }
@@ -460,26 +476,27 @@ struct Row {
     // list the candidates, in every CTA the same ones (in any order)
     if (tid == 0) s.n_cand = 0;
     lsync();
-    for (int i = tid; i < src.n; i += nt) {
-      const unsigned k = key_of(src.value(i));
-      if (k > lo && k <= hi) s.cand[atomicAdd(&s.n_cand, 1u)] = value_of(k);
+    for (int i = tid; i < src.n; i += nt()) {
+      const float v = src.value(i);
+      if (v >= lo && v <= hi) s.cand[atomicAdd(&s.n_cand, 1u)] = v;
     }
     gsync();
     unsigned n_all = 0;
     for (unsigned r = 0; r < (MODE == CLUSTER ? size : 1); r++) {
       const unsigned m = *peer(&s.n_cand, r);
       const float *c = peer(s.cand, r);
-      for (unsigned i = tid; i < m; i += nt) {
+      for (unsigned i = tid; i < m; i += nt()) {
         s.all[n_all + i] = c[i];
         if (BY_WEIGHT) s.all_w[n_all + i] = weight(c[i]);
       }
       n_all += m;
     }
     lsync();
-    for (unsigned i = tid; i < n_all; i += nt) {
+    for (unsigned i = tid; i < n_all; i += nt()) {
       const float v = s.all[i];
       u64 more = 0;         // count or weight of the larger ones
       unsigned ties = 0;
+#pragma unroll 4
       for (unsigned j = 0; j < n_all; j++) {
         const float o = s.all[j];
         ties += o == v;
@@ -487,7 +504,7 @@ struct Row {
       }
       const u64 each = BY_WEIGHT ? s.all_w[i] : 1, start = before + more;
       if (start < target && target <= start + each * ties) {   // equals write the same
-        s.cut_key = key_of(v);
+        s.cut = v;
         s.cut_ties = ties;
         s.cut_take = (unsigned)((target - start + each - 1) / each);
       }
@@ -495,72 +512,160 @@ struct Row {
     gsync();   // (cluster: the candidates are read)
   }
 
-  // The entries with key >= cut into the list, in index order, where every CTA's fit.
-  template <typename Src>
-  __device__ bool make_list(const Src &src, unsigned cut, FromList &out) {
-    const int per = ((src.n + nt - 1) / nt) | 1;   // odd: no bank conflicts between the threads' runs
-    const int i0 = min(tid * per, src.n), i1 = min(i0 + per, src.n);
-    unsigned c = 0;
-    for (int i = i0; i < i1; i++) c += key_of(src.value(i)) >= cut;
-    u64 all, most;
-    u64 at = scan<true>(c, all, most);
-    if (most > (u64)S::CAP) return false;
-    if (c)
-      for (int i = i0; i < i1; i++) {
-        const float v = src.value(i);
-        if (key_of(v) >= cut) {
-          s.list[at] = v;
-          s.index[at] = src.index(i);
-          at++;
+  // The row's entries >= edge (finite) into the list, in index order, where every
+  // CTA's fit.
+  __device__ bool make_list(const FromRow &src, float edge, FromList &out) {
+    const int lane = threadIdx.x & 31;
+    edge = fmaxf(edge, -3.402823466e38f);
+    // eight groups of 32 entries at a time, so that their reads and votes overlap
+    constexpr int G = 8;
+    // a contiguous segment per warp
+    const int warp = MODE == WARP ? 0 : threadIdx.x >> 5, nw = MODE == WARP ? 1 : (int)(blockDim.x >> 5);
+    const int per = ((src.n + nw - 1) / nw + 31) & ~31, i0 = min(warp * per, src.n), i1 = min(i0 + per, src.n);
+    unsigned at = 0;
+    if (MODE != WARP) {   // where this warp's part begins
+      unsigned c = 0;
+#pragma unroll 8
+      for (int i = i0 + lane; i < i1; i += 32) c += src.value(i) >= edge;
+      c = __reduce_add_sync(PK_FULL_MASK, c);
+      u64 all, most;
+      const u64 b = scan<true>(lane == 0 ? c : 0, all, most);
+      at = (unsigned)__shfl_sync(PK_FULL_MASK, b, 0);
+      if (most > (u64)S::CAP) return false;
+      if (threadIdx.x == blockDim.x - 32) s.n_cand = at + c;
+      if (c == 0) at = S::CAP;   // nothing to write
+    }
+    if (MODE == WARP || at < (unsigned)S::CAP)
+      for (int i = i0 + lane; i - lane < i1; i += 32 * G) {
+        float v[G];
+        unsigned who[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) v[g] = i + 32 * g < i1 ? src.value(i + 32 * g) : -INFINITY;
+#pragma unroll
+        for (int g = 0; g < G; g++) who[g] = __ballot_sync(PK_FULL_MASK, v[g] >= edge);
+        unsigned end = at;
+#pragma unroll
+        for (int g = 0; g < G; g++) end += __popc(who[g]);
+        if (MODE == WARP && end > (unsigned)S::CAP) return false;
+        if (end == at) continue;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          if (v[g] >= edge) {
+            const unsigned o = at + __popc(who[g] & ((1u << lane) - 1));
+            s.list[o] = v[g];
+            s.index[o] = src.index(i + 32 * g);
+          }
+          at += __popc(who[g]);
         }
       }
+    if (MODE == WARP) {
+      out.n = (int)at;
+      __syncwarp();
+    } else {
+      __syncthreads();
+      out.n = (int)s.n_cand;
+      __syncthreads();
+    }
     out.x = s.list;
     out.at = s.index;
-    // this CTA's own number: the last thread's end
-    if (tid == nt - 1) s.n_cand = (unsigned)at;
-    lsync();
-    out.n = (int)s.n_cand;
-    lsync();
     return true;
   }
 
-  // What the filters leave of a source, and the draw from it. Kept are keys > cut
-  // and the first `take` of its `ties` equals.
+  // Kept are values > v and the first `take` of the `ties` equal to it.
+  struct Cut {
+    float v;
+    unsigned take, ties;
+  };
+  __device__ __forceinline__ Cut read_cut() const { return Cut{s.cut, s.cut_take, s.cut_ties}; }
+
+  // The weights of the values > cut, and their bins in units of which the row's
+  // total fits 32 bits.
   template <typename Src>
-  __device__ void top_p_and_draw(const Src &src, long long row, unsigned cut, unsigned take, unsigned ties, float p,
-                                 float mp, double temp);
+  __device__ __forceinline__ u64 weigh(const Src &src, float cut) {
+    clear_bins();
+    Sums t = no_sums();
+    constexpr int G = 4;
+    for (int i = tid; i < src.n; i += G * nt()) {
+      float v[G];
+      u64 w[G];
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        v[g] = i + g * nt() < src.n ? src.value(i + g * nt()) : -INFINITY;
+        w[g] = weight(v[g]);
+      }
+#pragma unroll
+      for (int g = 0; g < G; g++)
+        if (v[g] > cut) {
+          t.w += w[g];
+          atomicAdd(&s.bins[bin_of(v[g])], (unsigned)((w[g] + (1ull << hint >> 1)) >> hint));
+        }
+    }
+    return total<true, false, false>(t).w;
+  }
+  // The least integer that is at least p times the sum (and at least 1).
+  __device__ __forceinline__ static u64 share(float p, u64 sum) {
+    const u64 t = p > 0.0f ? (u64)ceil((double)p * (double)sum) : 1;
+    return t < 1 ? 1 : t < sum ? t : sum;
+  }
+  __device__ __forceinline__ int find_weight(u64 target) {
+    unsigned before, inside;
+    u64 all;
+    const u64 goal = target >> hint;
+    return find_bin(goal ? goal : 1, before, inside, all);
+  }
   template <typename Src>
-  __device__ void draw(const Src &src, long long row, unsigned cut, unsigned take, unsigned ties, float mp, double temp);
+  __device__ __forceinline__ Cut top_p(const Src &src, Cut cut, float p) {
+    const u64 w = weigh(src, cut.v);
+    const u64 each = cut.ties ? weight(cut.v) : 0;
+    const u64 target = share(p, w + cut.take * each);
+    if (target > w) {   // inside the equals of the top-k's border
+      cut.take = (unsigned)((target - w + each - 1) / each);
+      return cut;
+    }
+    border<true>(src, cut.v, target, find_weight(target), 0, 0);
+    return read_cut();
+  }
+  template <typename Src>
+  __device__ void draw(const Src &src, long long row, Cut cut, float mp, float temp);
   __device__ void run(long long row);
 };
 
 template <typename T, int MODE>
 template <typename Src>
-__device__ void Row<T, MODE>::draw(const Src &src, long long row, unsigned cut, unsigned take, unsigned ties, float mp,
-                                   double temp) {
+__device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float mp, float temp) {
   const int lane = threadIdx.x & 31;
   // min-p: a weight at least min_p of the largest, which always stays
   u64 least = 0;
   if (mp > 0.0f) least = (u64)ceil((double)(mp < 1.0f ? mp : 1.0f) * 0x1p44);
-  const int per = ((src.n + nt - 1) / nt) | 1;
+  // a contiguous run of entries per thread, of odd length: no bank conflicts between the threads
+  const int per = ((src.n + nt() - 1) / nt()) | 1;
   const int i0 = min(tid * per, src.n), i1 = min(i0 + per, src.n);
-  const bool part = take < ties;
+  const bool part = cut.take < cut.ties;
+  const float low = cut.ties ? cut.v : -3.402823466e38f;   // kept are values >= low
   unsigned tie0 = 0;   // equals of the cut before this thread's run
   if (part) {
     unsigned c = 0;
-    for (int i = i0; i < i1; i++) c += key_of(src.value(i)) == cut;
+    for (int i = i0; i < i1; i++) c += src.value(i) == low;
     u64 all, most;
     tie0 = (unsigned)scan<false>(c, all, most);
   }
   u64 mine = 0;
   unsigned seen = tie0;
-  for (int i = i0; i < i1; i++) {
-    const float v = src.value(i);
-    const unsigned k = key_of(v);
-    if (k < cut || k == 0) continue;
-    if (k == cut && part && seen++ >= take) continue;
-    const u64 w = weight(v);
-    mine += w >= least ? w : 0;
+  constexpr int G = 6;
+  for (int i = i0; i < i1; i += G) {
+    float v[G];
+    u64 w[G];
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      v[j] = i + j < i1 ? src.value(i + j) : -INFINITY;
+      w[j] = weight(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      bool keep = v[j] >= low && w[j] >= least;
+      if (part && v[j] == low) keep = keep && seen++ < cut.take;
+      mine += keep ? w[j] : 0;
+    }
   }
   u64 sum, most;
   const u64 before = scan<false>(mine, sum, most);
@@ -577,15 +682,14 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, unsigned cut, 
   for (int j = j0; j < j1; j += 32) {
     const int i = j + lane;
     const float v = i < j1 ? src.value(i) : -INFINITY;
-    const unsigned k = key_of(v);
-    bool keep = k > cut || (k == cut && k != 0);
+    bool keep = v >= low;
     if (part) {
-      const unsigned same = __ballot_sync(PK_FULL_MASK, k == cut);
-      if (k == cut) keep = seen + __popc(same & ((1u << lane) - 1)) < take;
+      const unsigned same = __ballot_sync(PK_FULL_MASK, v == low);
+      if (v == low) keep = seen + __popc(same & ((1u << lane) - 1)) < cut.take;
       seen += __popc(same);
     }
-    u64 w = keep ? weight(v) : 0;
-    w = w >= least ? w : 0;
+    u64 w = weight(v);
+    w = keep && w >= least ? w : 0;
     const u64 inc = warp_scan_u64(w);
     const unsigned past = __ballot_sync(PK_FULL_MASK, run + inc > target);
     if (past) {
@@ -593,7 +697,7 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, unsigned cut, 
         a.tokens[row] = src.index(i);
         if (a.logprobs) {
           // log(w / S): the exponent itself less log S, S in units of the largest weight
-          const double y = v == max ? 0.0 : ((double)v - (double)max) / temp;
+          const double y = v == weight.max ? 0.0 : ((double)v - weight.top) / (double)temp;
           const double over = (double)(sum - (1ull << 44)) * 0x1p-44;
           a.logprobs[row] = (float)(y - (double)log1pf((float)over));
         }
@@ -605,61 +709,19 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, unsigned cut, 
 }
 
 template <typename T, int MODE>
-template <typename Src>
-__device__ void Row<T, MODE>::top_p_and_draw(const Src &src, long long row, unsigned cut, unsigned take, unsigned ties,
-                                             float p, float mp, double temp) {
-  if (p < 1.0f) {
-    clear_bins();
-    Sums t = no_sums();
-    for (int i = tid; i < src.n; i += nt) {
-      const float v = src.value(i);
-      const unsigned k = key_of(v);
-      if (k <= cut) continue;
-      const u64 w = weight(v);
-      t.w += w;
-      atomicAdd(&s.mass[bin_of(k)], (float)w * 0x1p-44f);
-    }
-    t = total<true, false, false>(t);
-    const u64 each = cut ? weight(value_of(cut)) : 0;
-    const u64 sum = t.w + take * each;
-    // the least integer that is at least p times the sum (and at least 1)
-    u64 target = p > 0.0f ? (u64)ceil((double)p * (double)sum) : 1;
-    target = target < 1 ? 1 : target < sum ? target : sum;
-    if (target > t.w) {   // inside the equals of the top-k's border
-      take = (unsigned)((target - t.w + each - 1) / each);
-    } else {
-      unsigned before, inside;
-      const int bin = find_bin<true>(target, before, inside);
-      // from here on only the entries of the bins up to that one count, and where
-      // they are few only they are looked at: keys from the bin's lower edge on
-      border<true>(src, cut, target, bin, 0, 0);
-      cut = s.cut_key;
-      take = s.cut_take;
-      ties = s.cut_ties;
-    }
-  }
-  draw(src, row, cut, take, ties, mp, temp);
-}
-
-template <typename T, int MODE>
 __device__ void Row<T, MODE>::run(long long row) {
   const T *in = static_cast<const T *>(a.logits) + row * a.ld + base;
   // the row, once; its largest and smallest values
   Sums v = no_sums();
-#pragma unroll 8
-  for (int i = tid; i < n; i += nt) {
-    const T e = in[i];
+#pragma unroll 16
+  for (int i = tid; i < n; i += nt()) {
+    const float e = clean(to_f32(in[i]));
     x[i] = e;
-    const unsigned k = key_of(to_f32(e));
-    if (k) {
-      v.lo = min(v.lo, k);
-      v.hi = ::max(v.hi, k);
-      v.n++;
-    }
+    v.hi = fmaxf(v.hi, e);
+    v.lo = fminf(v.lo, e == -INFINITY ? INFINITY : e);
   }
-  v = total<false, true, true>(v);
-  const unsigned max_key = v.hi;
-  if (v.n == 0) {   // nothing to take
+  v = total<false, false, true>(v);
+  if (v.hi == -INFINITY) {   // nothing to take
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
       if (a.logprobs) a.logprobs[row] = -INFINITY;
@@ -667,13 +729,14 @@ __device__ void Row<T, MODE>::run(long long row) {
     return;
   }
   lsync();
-  FromRow<T> all{x, n, base};
-  max = value_of(max_key);
+  const FromRow all{x, n, base};
   const float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
   if (!(temp > 0.0f)) {   // greedy: the first largest
+    unsigned first = 0xffffffffu;
+    for (int i = tid; i < n; i += nt())
+      if (x[i] == v.hi) first = min(first, (unsigned)(base + i));
     Sums f = no_sums();
-    for (int i = tid; i < n; i += nt)
-      if (key_of(all.value(i)) == max_key) f.lo = min(f.lo, (unsigned)(base + i));
+    f.lo = first == 0xffffffffu ? INFINITY : (float)first;   // indices below 2^18 are exact
     f = total<false, false, true>(f);
     if (rank == 0 && tid == 0) {
       a.tokens[row] = (int)f.lo;
@@ -681,32 +744,65 @@ __device__ void Row<T, MODE>::run(long long row) {
     }
     return;
   }
-  weight.c = 16.0 * 1.44269504088896340736 / (double)temp;
-  weight.max = max;
+  if (v.hi == INFINITY) {   // infinite ones share everything: they are zeros, the rest is masked
+    for (int i = tid; i < n; i += nt()) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+    v.hi = v.lo = 0.0f;
+    lsync();
+  }
+  weight.set(v.hi, temp);
   const int k = a.top_k ? __ldg(a.top_k + row) : 0;
   const float p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
   const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   // bins over the values' range, at most 64 wide (below it one open bin)
-  float range = max - value_of(v.lo);
+  float range = __fsub_rn(v.hi, v.lo);
   range = range < 64.0f ? range : 64.0f;
   scale = (float)(S::NB - 2) / fmaxf(range, 1e-30f);
-  if (k > 0 && (unsigned)k < v.n) {
+  Cut cut = {-INFINITY, 0, 0};
+  FromList few;
+  if (k > 0) {
     clear_bins();
-    for (int i = tid; i < n; i += nt) {
-      const unsigned e = key_of(all.value(i));
-      if (e) atomicAdd(&s.cnt[bin_of(e)], 1u);
+#pragma unroll 8
+    for (int i = tid; i < n; i += nt()) {
+      const float e = x[i];
+      if (e > -INFINITY) atomicAdd(&s.bins[bin_of(e)], 1u);
     }
     unsigned before, inside;
-    const int bin = find_bin<false>((u64)k, before, inside);
-    border<false>(all, 0, (u64)k, bin, before, inside);
-    const unsigned cut = s.cut_key, take = s.cut_take, ties = s.cut_ties;
-    lsync();
-    FromList few;
-    if (make_list(all, cut, few)) top_p_and_draw(few, row, cut, take, ties, p, mp, (double)temp);
-    else top_p_and_draw(all, row, cut, take, ties, p, mp, (double)temp);
-  } else {
-    top_p_and_draw(all, row, 0, 0, 0, p, mp, (double)temp);
+    u64 count;
+    const int bin = find_bin((u64)k, before, inside, count);
+    if ((u64)k < count) {
+      // of a list of the bins up to the border's, or of the row
+      if (before + inside <= (unsigned)S::CAP && make_list(all, edge_of(bin), few)) {
+        border<false>(few, -INFINITY, (u64)k, bin, before, inside);
+        cut = read_cut();
+        if (p < 1.0f) cut = top_p(few, cut, p);
+        draw(few, row, cut, mp, temp);
+        return;
+      }
+      border<false>(all, -INFINITY, (u64)k, bin, before, inside);
+      cut = read_cut();
+      if (p < 1.0f) cut = top_p(all, cut, p);
+      draw(all, row, cut, mp, temp);
+      return;
+    }
   }
+  if (p < 1.0f) {
+    const u64 target = share(p, weigh(all, -INFINITY));
+    int bin = find_weight(target);
+    for (int tries = 0; tries < 2 && make_list(all, edge_of(bin), few); tries++, bin = min(bin + 1, S::NB - 1)) {
+      Sums t = no_sums();
+      for (int i = tid; i < few.n; i += nt()) {
+        const float e = few.value(i);
+        if (bin_of(e) <= bin) t.w += weight(e);
+      }
+      if (total<true, false, false>(t).w < target) continue;   // a rounding of the hint: one bin more
+      border<true>(few, -INFINITY, target, bin, 0, 0);
+      draw(few, row, read_cut(), mp, temp);
+      return;
+    }
+    border<true>(all, -INFINITY, target, bin, 0, 0);
+    cut = read_cut();
+  }
+  draw(all, row, cut, mp, temp);
 }
 
 template <typename T, int MODE>
@@ -717,11 +813,12 @@ __global__ void __launch_bounds__(MODE == WARP ? 256 : 1024) sample_kernel(Args 
   if (threadIdx.x < 16) tab[threadIdx.x] = kPow2[threadIdx.x];
   __syncthreads();
   const int warp = threadIdx.x >> 5;
-  const size_t group = sizeof(S) + (((size_t)a.seg * sizeof(T) + 15) & ~(size_t)15);
+  const size_t group = sizeof(S) + (((size_t)a.seg * 4 + 15) & ~(size_t)15);
   unsigned char *mem = smem + (MODE == WARP ? warp * group : 0);
   S &s = *reinterpret_cast<S *>(mem);
   Row<T, MODE> r{a, s};
-  r.x = reinterpret_cast<T *>(mem + sizeof(S));
+  r.x = reinterpret_cast<float *>(mem + sizeof(S));
+  r.hint = 44 - 31 + (32 - __clz(a.V));   // V < 2^(32 - clz) weights of 2^44: 31 bits
   r.weight.tab = tab;
   r.flip = r.cflip = 0;
   r.size = MODE == CLUSTER ? cg::this_cluster().num_blocks() : 1;
@@ -730,7 +827,6 @@ __global__ void __launch_bounds__(MODE == WARP ? 256 : 1024) sample_kernel(Args 
   r.n = a.V - r.base < a.seg ? a.V - r.base : a.seg;
   if (r.n < 0) r.n = 0;
   r.tid = MODE == WARP ? threadIdx.x & 31 : threadIdx.x;
-  r.nt = MODE == WARP ? 32 : blockDim.x;
   const long long step = MODE == WARP ? (long long)gridDim.x * (blockDim.x >> 5) : gridDim.x / r.size;
   for (long long row = MODE == WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x / r.size;
        row < a.n_rows; row += step) {
@@ -744,7 +840,7 @@ int launch(Args a, int size, int threads, cudaStream_t s) {
   static int flags[64];
   a.seg = MODE == CLUSTER ? ((a.V + size - 1) / size + 31) & ~31 : a.V;
   const int groups = MODE == WARP ? threads / 32 : 1;
-  const size_t bytes = groups * (sizeof(Shared<MODE>) + (((size_t)a.seg * sizeof(T) + 15) & ~(size_t)15));
+  const size_t bytes = groups * (sizeof(Shared<MODE>) + (((size_t)a.seg * 4 + 15) & ~(size_t)15));
   smem_optin(sample_kernel<T, MODE>, 200 * 1024, flags);
   const long long most = 1 << 20;
   const long long rows = (a.n_rows + groups - 1) / groups;
@@ -773,7 +869,7 @@ int launch_rows(const Args &a, cudaStream_t s) {
   if (mode == 0 || (mode < 0 && a.V <= 2048 && a.n_rows > pkcu_sm_count())) return launch<T, WARP>(a, 1, mode < 0 ? 256 : threads, s);
   if (mode < 0) {
     // CTAs per row: what the logits need, and more while that leaves SMs idle
-    while ((((a.V + size - 1) / size + 31) & ~31) * (long long)sizeof(T) > SMEM_LOGITS) size *= 2;
+    while ((((a.V + size - 1) / size + 31) & ~31) * 4LL > SMEM_VALUES) size *= 2;
     while (size < 8 && a.n_rows * size * 2 <= pkcu_sm_count() && a.V / size > 4096) size *= 2;
     const int each = (a.V + size - 1) / size;
     threads = each <= 2048 ? 128 : each <= 8192 ? 512 : 1024;
