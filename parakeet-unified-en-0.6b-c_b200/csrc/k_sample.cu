@@ -94,7 +94,8 @@ struct Weight {
     c = 16.0 * 1.44269504088896340736 / (double)temp;
     least = __fsub_rn(m, __fmul_rn(41.6f, temp));   // 60 ln 2 = 41.59; rounds to a float no entry lies between
   }
-  __device__ __forceinline__ u64 operator()(float v) const {
+  // For v >= least (else any number).
+  __device__ __forceinline__ u64 raw(float v) const {
     const double d = __dadd_rn((double)v, -top);
     constexpr double kShift = 6755399441055744.0;   // 1.5 2^52
     const double t = fma(d, c, kShift);
@@ -105,12 +106,14 @@ struct Weight {
     double p = fma(fma(r, L * L * L * L * L / 120, L * L * L * L / 24), r2, fma(r, L * L * L / 6, L * L / 2));
     p = fma(p, r2, fma(r, L, 1.0));
     const double w = __dmul_rn(tab[n & 15], p);
-    // times 2^(n div 16 + 44), then to an integer
+    // times 2^(n div 16 + 44), then to an integer: the mantissa after adding 2^52
     const double s = __hiloint2double(__double2hiint(w) + (((n >> 4) + 44) << 20), __double2loint(w));
-    const double q = __dadd_rn(s, 4503599627370496.0);   // + 2^52
-    const bool in = v >= least;
-    const unsigned hi = in ? (unsigned)__double2hiint(q) & 0xfffffu : 0, lo = in ? (unsigned)__double2loint(q) : 0;
-    return (u64)hi << 32 | lo;
+    return (u64)__double_as_longlong(__dadd_rn(s, 4503599627370496.0)) - 0x4330000000000000ull;
+  }
+  __device__ __forceinline__ u64 operator()(float v) const { return v >= least ? raw(v) : 0; }
+  // (v - max) / T
+  __device__ __forceinline__ double exponent(float v) const {
+    return __dmul_rn(__dmul_rn(__dadd_rn((double)v, -top), c), 0.693147180559945309417 / 16);
   }
 };
 
@@ -173,7 +176,8 @@ struct FromRow {
 struct FromList {
   const float *x;
   const int *at;
-  int n;
+  int n;       // this CTA's
+  int total;   // the row's (not kept for a warp's)
   __device__ __forceinline__ float value(int i) const { return x[i]; }
   __device__ __forceinline__ int index(int i) const { return at[i]; }
 };
@@ -323,6 +327,10 @@ struct Row {
   __device__ __forceinline__ float edge_of(int bin) const {
     return bin >= S::NB - 1 ? -INFINITY : __fsub_rn(weight.max, __fdiv_rn((float)bin + 0.6f, scale));
   }
+  // Bins from the maximum down to `lowest`, at least.
+  __device__ __forceinline__ void set_scale(float lowest) {
+    scale = (float)(S::NB - 2) / fmaxf(__fsub_rn(weight.max, lowest), 1e-30f);
+  }
   __device__ __forceinline__ void clear_bins() {
     lsync();
     for (int b = tid; b < S::NB; b += nt()) s.bins[b] = 0;
@@ -468,7 +476,7 @@ struct Row {
         const u64 each = BY_WEIGHT ? weight(hi) : 1;
         s.cut = hi;
         s.cut_ties = inside;
-        s.cut_take = (unsigned)((target - before + each - 1) / each);
+        s.cut_take = (unsigned)(BY_WEIGHT ? (target - before + each - 1) / each : target - before);
       }
       lsync();
       return;
@@ -506,7 +514,7 @@ struct Row {
       if (start < target && target <= start + each * ties) {   // equals write the same
         s.cut = v;
         s.cut_ties = ties;
-        s.cut_take = (unsigned)((target - start + each - 1) / each);
+        s.cut_take = ties == 1 ? 1 : (unsigned)(BY_WEIGHT ? (target - start + each - 1) / each : target - start);
       }
     }
     gsync();   // (cluster: the candidates are read)
@@ -517,58 +525,84 @@ struct Row {
   __device__ bool make_list(const FromRow &src, float edge, FromList &out) {
     const int lane = threadIdx.x & 31;
     edge = fmaxf(edge, -3.402823466e38f);
-    // eight groups of 32 entries at a time, so that their reads and votes overlap
-    constexpr int G = 8;
-    // a contiguous segment per warp
-    const int warp = MODE == WARP ? 0 : threadIdx.x >> 5, nw = MODE == WARP ? 1 : (int)(blockDim.x >> 5);
-    const int per = ((src.n + nw - 1) / nw + 31) & ~31, i0 = min(warp * per, src.n), i1 = min(i0 + per, src.n);
-    unsigned at = 0;
-    if (MODE != WARP) {   // where this warp's part begins
+    if constexpr (MODE == WARP) {
+      // a contiguous run per lane, of odd length (no bank conflicts), at most 63: which
+      // of its entries belong, as bits; reads past the run's end are masked
+      const int per = ((src.n + 31) / 32) | 1, i0 = min(lane * per, src.n), len = min(per, src.n - i0);
+      u64 in = 0;
+      for (int j = 0; j < per; j += 8) {
+        unsigned m = 0;
+#pragma unroll
+        for (int g = 0; g < 8; g++) m |= src.value(lane * per + j + g) >= edge ? 1u << g : 0;
+        in |= (u64)m << j;
+      }
+      in &= (1ull << len) - 1;
+      const unsigned c = __popcll(in);
+      unsigned end = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned up = __shfl_up_sync(PK_FULL_MASK, end, o);
+        if (lane >= o) end += up;
+      }
+      out.n = (int)__shfl_sync(PK_FULL_MASK, end, 31);
+      if (out.n > S::CAP) return false;
+      for (unsigned at = end - c; in; in &= in - 1, at++) {
+        const int i = i0 + __ffsll((long long)in) - 1;
+        s.list[at] = src.value(i);
+        s.index[at] = src.index(i);
+      }
+      __syncwarp();
+    } else {
+      // a contiguous segment per warp; eight groups of 32 entries at a time, so that
+      // their reads and votes overlap
+      constexpr int G = 8;
+      const int warp = threadIdx.x >> 5, nw = (int)(blockDim.x >> 5);
+      const int per = ((src.n + nw - 1) / nw + 31) & ~31, i0 = min(warp * per, src.n), i1 = min(i0 + per, src.n);
       unsigned c = 0;
 #pragma unroll 8
       for (int i = i0 + lane; i < i1; i += 32) c += src.value(i) >= edge;
       c = __reduce_add_sync(PK_FULL_MASK, c);
       u64 all, most;
       const u64 b = scan<true>(lane == 0 ? c : 0, all, most);
-      at = (unsigned)__shfl_sync(PK_FULL_MASK, b, 0);
+      unsigned at = (unsigned)__shfl_sync(PK_FULL_MASK, b, 0);
       if (most > (u64)S::CAP) return false;
       if (threadIdx.x == blockDim.x - 32) s.n_cand = at + c;
-      if (c == 0) at = S::CAP;   // nothing to write
-    }
-    if (MODE == WARP || at < (unsigned)S::CAP)
-      for (int i = i0 + lane; i - lane < i1; i += 32 * G) {
-        float v[G];
-        unsigned who[G];
+      if (c)
+        for (int i = i0 + lane; i - lane < i1; i += 32 * G) {
+          float v[G];
+          unsigned who[G];
 #pragma unroll
-        for (int g = 0; g < G; g++) v[g] = i + 32 * g < i1 ? src.value(i + 32 * g) : -INFINITY;
+          for (int g = 0; g < G; g++) v[g] = i + 32 * g < i1 ? src.value(i + 32 * g) : -INFINITY;
 #pragma unroll
-        for (int g = 0; g < G; g++) who[g] = __ballot_sync(PK_FULL_MASK, v[g] >= edge);
-        unsigned end = at;
+          for (int g = 0; g < G; g++) who[g] = __ballot_sync(PK_FULL_MASK, v[g] >= edge);
 #pragma unroll
-        for (int g = 0; g < G; g++) end += __popc(who[g]);
-        if (MODE == WARP && end > (unsigned)S::CAP) return false;
-        if (end == at) continue;
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          if (v[g] >= edge) {
-            const unsigned o = at + __popc(who[g] & ((1u << lane) - 1));
-            s.list[o] = v[g];
-            s.index[o] = src.index(i + 32 * g);
+          for (int g = 0; g < G; g++) {
+            if (!who[g]) continue;
+            if (v[g] >= edge) {
+              const unsigned o = at + __popc(who[g] & ((1u << lane) - 1));
+              s.list[o] = v[g];
+              s.index[o] = src.index(i + 32 * g);
+            }
+            at += __popc(who[g]);
           }
-          at += __popc(who[g]);
         }
-      }
-    if (MODE == WARP) {
-      out.n = (int)at;
-      __syncwarp();
-    } else {
       __syncthreads();
       out.n = (int)s.n_cand;
+      out.total = (int)all;
       __syncthreads();
     }
     out.x = s.list;
     out.at = s.index;
     return true;
+  }
+
+  __device__ bool small(const FromList &src, int n, long long row, int k, float p, u64 all_w, float mp, float uu);
+
+  // log(w / S) of a value: the exponent itself less log S, S in units of the
+  // largest weight (which is one of its parts).
+  __device__ __forceinline__ float log_prob(float v, u64 sum) const {
+    const double over = (double)(sum - (1ull << 44)) * 0x1p-44;
+    return (float)((v == weight.max ? 0.0 : weight.exponent(v)) - (double)log1pf((float)over));
   }
 
   // Kept are values > v and the first `take` of the `ties` equal to it.
@@ -578,28 +612,34 @@ struct Row {
   };
   __device__ __forceinline__ Cut read_cut() const { return Cut{s.cut, s.cut_take, s.cut_ties}; }
 
-  // The weights of the values > cut, and their bins in units of which the row's
-  // total fits 32 bits.
-  template <typename Src>
+  // The sum of the weights of the values > cut; BINS: their bins too, in units of
+  // which the row's total fits 32 bits.
+  template <bool BINS, typename Src>
   __device__ __forceinline__ u64 weigh(const Src &src, float cut) {
-    clear_bins();
+    if (BINS) clear_bins();
     Sums t = no_sums();
-    constexpr int G = 4;
-    for (int i = tid; i < src.n; i += G * nt()) {
+    constexpr int G = 6;
+    // at least the limit below which weights are 0, and past the cut
+    const float low = weight.least > cut ? weight.least : cut;
+    const bool past = low == cut;
+    auto group = [&](int i, bool whole) {
       float v[G];
       u64 w[G];
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        v[g] = i + g * nt() < src.n ? src.value(i + g * nt()) : -INFINITY;
-        w[g] = weight(v[g]);
+        v[g] = whole || i + g * nt() < src.n ? src.value(i + g * nt()) : -INFINITY;
+        w[g] = weight.raw(v[g]);
       }
 #pragma unroll
       for (int g = 0; g < G; g++)
-        if (v[g] > cut) {
+        if (past ? v[g] > low : v[g] >= low) {
           t.w += w[g];
-          atomicAdd(&s.bins[bin_of(v[g])], (unsigned)((w[g] + (1ull << hint >> 1)) >> hint));
+          if (BINS) atomicAdd(&s.bins[bin_of(v[g])], (unsigned)((w[g] + (1ull << hint >> 1)) >> hint));
         }
-    }
+    };
+    int i = tid;
+    for (; i + (G - 1) * nt() < src.n; i += G * nt()) group(i, true);
+    if (i < src.n) group(i, false);
     return total<true, false, false>(t).w;
   }
   // The least integer that is at least p times the sum (and at least 1).
@@ -615,7 +655,7 @@ struct Row {
   }
   template <typename Src>
   __device__ __forceinline__ Cut top_p(const Src &src, Cut cut, float p) {
-    const u64 w = weigh(src, cut.v);
+    const u64 w = weigh<true>(src, cut.v);
     const u64 each = cut.ties ? weight(cut.v) : 0;
     const u64 target = share(p, w + cut.take * each);
     if (target > w) {   // inside the equals of the top-k's border
@@ -626,13 +666,15 @@ struct Row {
     return read_cut();
   }
   template <typename Src>
-  __device__ void draw(const Src &src, long long row, Cut cut, float mp, float temp);
+  __device__ void draw(const Src &src, long long row, Cut cut, float mp, float uu);
+  template <typename Src>
+  __device__ __forceinline__ void count(const Src &src);
   __device__ void run(long long row);
 };
 
 template <typename T, int MODE>
 template <typename Src>
-__device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float mp, float temp) {
+__device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float mp, float uu) {
   const int lane = threadIdx.x & 31;
   // min-p: a weight at least min_p of the largest, which always stays
   u64 least = 0;
@@ -649,27 +691,36 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float
     u64 all, most;
     tie0 = (unsigned)scan<false>(c, all, most);
   }
+  const float low0 = fmaxf(low, weight.least);   // below it weights are 0
   u64 mine = 0;
   unsigned seen = tie0;
   constexpr int G = 6;
-  for (int i = i0; i < i1; i += G) {
+  auto group = [&](int i, bool whole) {
     float v[G];
     u64 w[G];
 #pragma unroll
     for (int j = 0; j < G; j++) {
-      v[j] = i + j < i1 ? src.value(i + j) : -INFINITY;
-      w[j] = weight(v[j]);
+      v[j] = whole || i + j < i1 ? src.value(i + j) : -INFINITY;
+      w[j] = weight.raw(v[j]);
     }
+    if (part || least) {
 #pragma unroll
-    for (int j = 0; j < G; j++) {
-      bool keep = v[j] >= low && w[j] >= least;
-      if (part && v[j] == low) keep = keep && seen++ < cut.take;
-      mine += keep ? w[j] : 0;
+      for (int j = 0; j < G; j++) {
+        bool keep = v[j] >= low0 && w[j] >= least;
+        if (part && v[j] == low) keep = keep && seen++ < cut.take;
+        if (keep) mine += w[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < G; j++)
+        if (v[j] >= low0) mine += w[j];
     }
-  }
+  };
+  int i = i0;
+  for (; i + G <= i1; i += G) group(i, true);
+  if (i < i1) group(i, false);
   u64 sum, most;
   const u64 before = scan<false>(mine, sum, most);
-  const float uu = __ldg(a.u + row);
   u64 target = uu > 0.0f ? (u64)((double)uu * (double)sum) : 0;   // floor; the running sum has to exceed it
   target = target < sum ? target : sum - 1;
   const unsigned owner = __ballot_sync(PK_FULL_MASK, target >= before && target < before + mine);
@@ -695,12 +746,7 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float
     if (past) {
       if (lane == __ffs(past) - 1) {
         a.tokens[row] = src.index(i);
-        if (a.logprobs) {
-          // log(w / S): the exponent itself less log S, S in units of the largest weight
-          const double y = v == weight.max ? 0.0 : ((double)v - weight.top) / (double)temp;
-          const double over = (double)(sum - (1ull << 44)) * 0x1p-44;
-          a.logprobs[row] = (float)(y - (double)log1pf((float)over));
-        }
+        if (a.logprobs) a.logprobs[row] = log_prob(v, sum);
       }
       break;
     }
@@ -708,18 +754,186 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float
   }
 }
 
+// Filters and draw for at most 256 listed entries, by one warp in its registers:
+// entry 32 j + lane is the lane's j-th. n: the list's length (all of the row's lists
+// in rank order, for a cluster's first warp). k > 0: the k largest of them; p < 1:
+// of these those whose weight reaches p times theirs, or times all_w where k is 0.
+// A border is found by halving the range of keys, counts and weights (in two
+// 22-bit halves, so that 256 of them fit a 32-bit reduction) summed exactly in
+// each step, until one entry is left in the range, or one key. False: the entries
+// weigh less than the share asked for, nothing is drawn.
+template <typename T, int MODE>
+__device__ bool Row<T, MODE>::small(const FromList &src, int n, long long row, int k, float p, u64 all_w, float mp,
+                                    float uu) {
+  constexpr int J = 8;
+  const int lane = threadIdx.x & 31;
+  unsigned key[J], wl[J], wh[J];   // key 0: dropped
+  int from[J];                     // (cluster) rank and place of the entry
+  unsigned lowest = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    const int i = 32 * j + lane;
+    float v = -INFINITY;
+    from[j] = i;
+    if (i < n) {
+      if (MODE == CLUSTER) {
+        unsigned r = 0;
+        int at = i;
+        for (; r < size - 1; r++) {
+          const int m = (int)*peer(&s.n_cand, r);
+          if (at < m) break;
+          at -= m;
+        }
+        v = *peer(&s.list[at], r);
+        from[j] = (int)(r << 16) | at;
+      } else {
+        v = src.x[i];
+      }
+    }
+    const u64 w = i < n ? weight(v) : 0;
+    key[j] = i < n ? key_of(v) : 0;
+    wl[j] = (unsigned)w & 0x3fffffu;
+    wh[j] = (unsigned)(w >> 22);
+    lowest = min(lowest, key[j] - 1);
+  }
+  lowest = __reduce_min_sync(PK_FULL_MASK, lowest);   // below every entry's key
+  const unsigned highest = key_of(weight.max);
+  auto count = [&](unsigned above) {
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < J; j++) c += key[j] > above;
+    return (int)__reduce_add_sync(PK_FULL_MASK, c);
+  };
+  auto mass = [&](unsigned above) {
+    unsigned l = 0, h = 0;
+#pragma unroll
+    for (int j = 0; j < J; j++)
+      if (key[j] > above) {
+        l += wl[j];
+        h += wh[j];
+      }
+    return ((u64)__reduce_add_sync(PK_FULL_MASK, h) << 22) + __reduce_add_sync(PK_FULL_MASK, l);
+  };
+  // keeps keys > above, and of those equal to it the first `take`
+  auto drop = [&](unsigned above, unsigned take) {
+    unsigned seen = 0;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      bool keep = key[j] > above;
+      if (take) {
+        const unsigned same = __ballot_sync(PK_FULL_MASK, key[j] == above);
+        if (key[j] == above) keep = seen + __popc(same & ((1u << lane) - 1)) < take;
+        seen += __popc(same);
+      }
+      if (!keep) key[j] = wl[j] = wh[j] = 0;
+    }
+  };
+  if (k > 0 && k < n) {
+    unsigned lo = lowest, hi = highest;   // count(lo) > k > count(hi)
+    for (;;) {
+      if (hi - lo == 1) {   // equals at the border
+        drop(hi, (unsigned)(k - count(hi)));
+        break;
+      }
+      const unsigned mid = lo + (hi - lo) / 2;
+      const int c = count(mid);
+      if (c == k) {
+        drop(mid, 0);
+        lo = mid;
+        break;
+      }
+      if (c > k) lo = mid;
+      else hi = mid;
+    }
+    lowest = lo;
+  }
+  if (p < 1.0f) {
+    const u64 have = mass(0);
+    const u64 target = share(p, k > 0 ? have : all_w);
+    if (have < target) return false;
+    unsigned lo = lowest, hi = highest;   // mass(lo) >= target > mass(hi)
+    int clo = count(lo), chi = 0;
+    for (;;) {
+      if (clo - chi == 1) {   // the border's entry alone
+        drop(lo, 0);
+        break;
+      }
+      if (hi - lo == 1) {   // equals at the border
+        const u64 each = weight(value_of(hi));
+        drop(hi, (unsigned)((target - mass(hi) + each - 1) / each));
+        break;
+      }
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (mass(mid) >= target) {
+        lo = mid;
+        clo = count(mid);
+      } else {
+        hi = mid;
+        chi = count(mid);
+      }
+    }
+  }
+  if (mp > 0.0f) {
+    const u64 least = (u64)ceil((double)(mp < 1.0f ? mp : 1.0f) * 0x1p44);
+#pragma unroll
+    for (int j = 0; j < J; j++)
+      if (((u64)wh[j] << 22) + wl[j] < least) key[j] = wl[j] = wh[j] = 0;
+  }
+  const u64 sum = mass(0);
+  u64 target = uu > 0.0f ? (u64)((double)uu * (double)sum) : 0;
+  target = target < sum ? target : sum - 1;
+  u64 run = 0;
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    const u64 part = ((u64)__reduce_add_sync(PK_FULL_MASK, wh[j]) << 22) + __reduce_add_sync(PK_FULL_MASK, wl[j]);
+    if (target < run + part) {
+      const u64 inc = warp_scan_u64(((u64)wh[j] << 22) + wl[j]);
+      const unsigned past = __ballot_sync(PK_FULL_MASK, run + inc > target);
+      if (lane == __ffs(past) - 1) {
+        a.tokens[row] = MODE == CLUSTER ? *peer(&s.index[from[j] & 0xffff], from[j] >> 16) : src.at[from[j]];
+        if (a.logprobs) a.logprobs[row] = log_prob(value_of(key[j]), sum);
+      }
+      break;
+    }
+    run += part;
+  }
+  return true;
+}
+
+// The counts of a source's entries per bin.
+template <typename T, int MODE>
+template <typename Src>
+__device__ __forceinline__ void Row<T, MODE>::count(const Src &src) {
+  clear_bins();
+#pragma unroll 8
+  for (int i = tid; i < src.n; i += nt()) {
+    const float e = src.value(i);
+    if (e > -INFINITY) atomicAdd(&s.bins[bin_of(e)], 1u);
+  }
+}
+
 template <typename T, int MODE>
 __device__ void Row<T, MODE>::run(long long row) {
   const T *in = static_cast<const T *>(a.logits) + row * a.ld + base;
-  // the row, once; its largest and smallest values
+  const float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
+  const int k = a.top_k ? __ldg(a.top_k + row) : 0;
+  const float p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
+  const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
+  const float uu = __ldg(a.u + row);
+  // the row, once; its largest value. Its smallest finite one for the bins; a warp
+  // takes instead the smallest of its lanes' second largest: some 150 to 200
+  // entries are as large, whatever the distribution, and mostly only they matter.
   Sums v = no_sums();
+  float second = -INFINITY;
 #pragma unroll 16
   for (int i = tid; i < n; i += nt()) {
     const float e = clean(to_f32(in[i]));
     x[i] = e;
+    if (MODE == WARP) second = fmaxf(second, fminf(v.hi, e));
+    else v.lo = fminf(v.lo, e == -INFINITY ? INFINITY : e);
     v.hi = fmaxf(v.hi, e);
-    v.lo = fminf(v.lo, e == -INFINITY ? INFINITY : e);
   }
+  if (MODE == WARP) v.lo = second;
   v = total<false, false, true>(v);
   if (v.hi == -INFINITY) {   // nothing to take
     if (rank == 0 && tid == 0) {
@@ -730,7 +944,6 @@ __device__ void Row<T, MODE>::run(long long row) {
   }
   lsync();
   const FromRow all{x, n, base};
-  const float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
   if (!(temp > 0.0f)) {   // greedy: the first largest
     unsigned first = 0xffffffffu;
     for (int i = tid; i < n; i += nt())
@@ -746,47 +959,58 @@ __device__ void Row<T, MODE>::run(long long row) {
   }
   if (v.hi == INFINITY) {   // infinite ones share everything: they are zeros, the rest is masked
     for (int i = tid; i < n; i += nt()) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
-    v.hi = v.lo = 0.0f;
+    v.hi = 0.0f;
+    v.lo = MODE == WARP ? -INFINITY : 0.0f;
     lsync();
   }
   weight.set(v.hi, temp);
-  const int k = a.top_k ? __ldg(a.top_k + row) : 0;
-  const float p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
-  const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
-  // bins over the values' range, at most 64 wide (below it one open bin)
-  float range = __fsub_rn(v.hi, v.lo);
-  range = range < 64.0f ? range : 64.0f;
-  scale = (float)(S::NB - 2) / fmaxf(range, 1e-30f);
   Cut cut = {-INFINITY, 0, 0};
   FromList few;
-  if (k > 0) {
-    clear_bins();
-#pragma unroll 8
-    for (int i = tid; i < n; i += nt()) {
-      const float e = x[i];
-      if (e > -INFINITY) atomicAdd(&s.bins[bin_of(e)], 1u);
+  unsigned before, inside;
+  u64 n_all;
+  const bool by_p = p < 1.0f;
+  if constexpr (MODE == WARP) {
+    if ((k > 0 || by_p) && make_list(all, v.lo, few)) {
+      const bool whole = v.lo == -INFINITY;   // the list is all that can be taken
+      if (k > 0 ? k <= few.n || whole : true) {
+        u64 all_w = 0;
+        if (by_p && k <= 0) all_w = whole ? weigh<false>(few, -INFINITY) : weigh<false>(all, -INFINITY);
+        if (small(few, few.n, row, k, p, all_w, mp, uu)) return;
+      }
     }
-    unsigned before, inside;
-    u64 count;
-    const int bin = find_bin((u64)k, before, inside, count);
-    if ((u64)k < count) {
+    if (k > 0 || by_p) {   // bins over the whole row
+      v.lo = INFINITY;
+      for (int i = tid; i < n; i += nt()) v.lo = fminf(v.lo, x[i] == -INFINITY ? INFINITY : x[i]);
+      v = total<false, false, true>(v);
+    }
+  }
+  set_scale(fmaxf(v.lo, __fsub_rn(v.hi, 64.0f)));
+  if (k > 0) {
+    count(all);
+    const int bin = find_bin((u64)k, before, inside, n_all);
+    if ((u64)k < n_all) {
       // of a list of the bins up to the border's, or of the row
       if (before + inside <= (unsigned)S::CAP && make_list(all, edge_of(bin), few)) {
+        if (MODE != WARP && few.total <= 256) {
+          gsync();   // every CTA's list is there
+          if (rank == 0 && threadIdx.x < 32) small(few, few.total, row, k, p, 0, mp, uu);
+          return;
+        }
         border<false>(few, -INFINITY, (u64)k, bin, before, inside);
         cut = read_cut();
-        if (p < 1.0f) cut = top_p(few, cut, p);
-        draw(few, row, cut, mp, temp);
+        if (by_p) cut = top_p(few, cut, p);
+        draw(few, row, cut, mp, uu);
         return;
       }
       border<false>(all, -INFINITY, (u64)k, bin, before, inside);
       cut = read_cut();
-      if (p < 1.0f) cut = top_p(all, cut, p);
-      draw(all, row, cut, mp, temp);
+      if (by_p) cut = top_p(all, cut, p);
+      draw(all, row, cut, mp, uu);
       return;
     }
   }
-  if (p < 1.0f) {
-    const u64 target = share(p, weigh(all, -INFINITY));
+  if (by_p) {
+    const u64 all_w = weigh<true>(all, -INFINITY), target = share(p, all_w);
     int bin = find_weight(target);
     for (int tries = 0; tries < 2 && make_list(all, edge_of(bin), few); tries++, bin = min(bin + 1, S::NB - 1)) {
       Sums t = no_sums();
@@ -795,25 +1019,36 @@ __device__ void Row<T, MODE>::run(long long row) {
         if (bin_of(e) <= bin) t.w += weight(e);
       }
       if (total<true, false, false>(t).w < target) continue;   // a rounding of the hint: one bin more
+      if (MODE != WARP && few.total <= 256) {
+        if (rank == 0 && threadIdx.x < 32) small(few, few.total, row, 0, p, all_w, mp, uu);
+        return;
+      }
       border<true>(few, -INFINITY, target, bin, 0, 0);
-      draw(few, row, read_cut(), mp, temp);
+      draw(few, row, read_cut(), mp, uu);
       return;
     }
     border<true>(all, -INFINITY, target, bin, 0, 0);
     cut = read_cut();
   }
-  draw(all, row, cut, mp, temp);
+  draw(all, row, cut, mp, uu);
 }
 
+// A group's shared memory; a warp reads up to 32 runs of odd length, and 8 more.
+template <int MODE>
+__host__ __device__ constexpr size_t group_bytes(int seg) {
+  return sizeof(Shared<MODE>) + (((size_t)(MODE == WARP ? ((seg + 31) / 32 | 1) * 32 + 8 : seg) * 4 + 15) & ~(size_t)15);
+}
+constexpr int WARP_MAX = 2016;   // entries of a warp's row: runs of 63
+
 template <typename T, int MODE>
-__global__ void __launch_bounds__(MODE == WARP ? 256 : 1024) sample_kernel(Args a) {
+__global__ void __launch_bounds__(MODE == WARP ? 256 : 1024, MODE == WARP ? 3 : 1) sample_kernel(Args a) {
   typedef Shared<MODE> S;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double tab[16];
   if (threadIdx.x < 16) tab[threadIdx.x] = kPow2[threadIdx.x];
   __syncthreads();
   const int warp = threadIdx.x >> 5;
-  const size_t group = sizeof(S) + (((size_t)a.seg * 4 + 15) & ~(size_t)15);
+  const size_t group = group_bytes<MODE>(a.seg);
   unsigned char *mem = smem + (MODE == WARP ? warp * group : 0);
   S &s = *reinterpret_cast<S *>(mem);
   Row<T, MODE> r{a, s};
@@ -840,7 +1075,7 @@ int launch(Args a, int size, int threads, cudaStream_t s) {
   static int flags[64];
   a.seg = MODE == CLUSTER ? ((a.V + size - 1) / size + 31) & ~31 : a.V;
   const int groups = MODE == WARP ? threads / 32 : 1;
-  const size_t bytes = groups * (sizeof(Shared<MODE>) + (((size_t)a.seg * 4 + 15) & ~(size_t)15));
+  const size_t bytes = groups * group_bytes<MODE>(a.seg);
   smem_optin(sample_kernel<T, MODE>, 200 * 1024, flags);
   const long long most = 1 << 20;
   const long long rows = (a.n_rows + groups - 1) / groups;
@@ -866,7 +1101,7 @@ int launch_rows(const Args &a, cudaStream_t s) {
   static const char *e = getenv("SMODE");
   int mode = -1, size = 1, threads = 0;
   if (e) sscanf(e, "%d,%d,%d", &mode, &size, &threads);
-  if (mode == 0 || (mode < 0 && a.V <= 2048 && a.n_rows > pkcu_sm_count())) return launch<T, WARP>(a, 1, mode < 0 ? 256 : threads, s);
+  if (mode == 0 || (mode < 0 && a.V <= WARP_MAX && a.n_rows > pkcu_sm_count())) return launch<T, WARP>(a, 1, mode < 0 ? 256 : threads, s);
   if (mode < 0) {
     // CTAs per row: what the logits need, and more while that leaves SMs idle
     while ((((a.V + size - 1) / size + 31) & ~31) * 4LL > SMEM_VALUES) size *= 2;
