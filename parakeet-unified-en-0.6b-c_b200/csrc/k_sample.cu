@@ -34,8 +34,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
-#include <stdio.h>
-#include <stdlib.h>
 
 #include "pk_common.cuh"
 #include "pk_types.cuh"
@@ -117,25 +115,47 @@ struct Weight {
   }
 };
 
-// A row's shared memory, per group (per CTA of a cluster).
+// A row's shared memory, per group (per CTA of a cluster). A warp's row uses its
+// list or its bins and candidates, never both.
 template <int MODE>
-struct Shared {
-  static constexpr int NB = MODE == WARP ? 256 : 1024;    // bins
+struct Listed {
   static constexpr int CAP = MODE == WARP ? 256 : 2048;   // entries of the list
+  float list[CAP];          // this CTA's: values and indices, in index order
+  int index[CAP];
+};
+template <int MODE>
+struct Binned {
+  static constexpr int NB = MODE == WARP ? 256 : 1024;    // bins
   static constexpr int RANK = MODE == WARP ? 64 : 512;    // candidates ranked against each other
-  static constexpr int NW = MODE == WARP ? 1 : 32;
-  u64 part_w[2][NW];        // a warp's part of a reduction or scan; alternating
-  unsigned part_n[2][NW];
-  float part_lo[2][NW], part_hi[2][NW];
-  u64 cta_w[2];             // this CTA's part, read by the cluster; alternating
-  unsigned cta_n[2];
-  float cta_lo[2], cta_hi[2];
   u64 all_w[RANK];
   float all[RANK];
   float cand[RANK];         // this CTA's candidates, read by the cluster
   unsigned bins[NB];        // counts, or weights in hint units
-  float list[CAP];          // this CTA's list: values and indices, in index order
-  int index[CAP];
+};
+template <int MODE>
+struct Both : Listed<MODE>, Binned<MODE> {};
+template <>
+struct Both<WARP> {
+  union {
+    struct {
+      float list[Listed<WARP>::CAP];
+      int index[Listed<WARP>::CAP];
+    };
+    struct {
+      u64 all_w[Binned<WARP>::RANK];
+      float all[Binned<WARP>::RANK], cand[Binned<WARP>::RANK];
+      unsigned bins[Binned<WARP>::NB];
+    };
+  };
+};
+template <int MODE>
+struct Shared : Both<MODE> {
+  static constexpr int NB = Binned<MODE>::NB, CAP = Listed<MODE>::CAP, RANK = Binned<MODE>::RANK;
+  static constexpr int NW = MODE == WARP ? 1 : 32;
+  u64 part_w[2][NW], part_w2[2][NW];   // a warp's part of a reduction or scan; alternating
+  unsigned part_n[2][NW], part_lo[2][NW], part_hi[2][NW];
+  u64 cta_w[2], cta_w2[2];             // this CTA's part, read by the cluster; alternating
+  unsigned cta_n[2], cta_lo[2], cta_hi[2];
   unsigned n_cand;
   int bin;
   unsigned bin_before, bin_inside;
@@ -145,16 +165,18 @@ struct Shared {
 
 // Sums and extremes over a row's entries.
 struct Sums {
-  u64 w;         // weights
+  u64 w, w2;     // weights
   unsigned n;    // entries
   float lo, hi;  // smallest, largest value
 };
-__device__ __forceinline__ Sums no_sums() { return Sums{0, 0, INFINITY, -INFINITY}; }
+__device__ __forceinline__ Sums no_sums() { return Sums{0, 0, 0, INFINITY, -INFINITY}; }
 
+// (three 22-bit parts, whose sums over 32 lanes fit 27 bits; v < 2^66)
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(PK_FULL_MASK, v, o);
-  return v;
+  const unsigned a = __reduce_add_sync(PK_FULL_MASK, (unsigned)v & 0x3fffffu);
+  const unsigned b = __reduce_add_sync(PK_FULL_MASK, (unsigned)(v >> 22) & 0x3fffffu);
+  const unsigned c = __reduce_add_sync(PK_FULL_MASK, (unsigned)(v >> 44));
+  return a + ((u64)b << 22) + ((u64)c << 44);
 }
 __device__ __forceinline__ u64 warp_scan_u64(u64 v) {   // inclusive
   const int lane = threadIdx.x & 31;
@@ -211,69 +233,72 @@ struct Row {
     return MODE == CLUSTER ? cg::this_cluster().map_shared_rank(p, r) : p;
   }
 
-  // Totals over the row's threads, to every thread. What is asked for: W weights,
-  // N entries, K extreme values.
-  template <bool W, bool N, bool K>
+  // Totals over the row's threads, to every thread. What is asked for: W weights
+  // (1 or 2 sums), N entries, K extreme values (reduced as keys).
+  template <int W, bool N, bool K>
   __device__ __forceinline__ Sums total(Sums v) {
     const int lane = threadIdx.x & 31;
-    reduce<W, N, K>(v);
+    unsigned lo = K ? key_of(v.lo) : 0, hi = K ? key_of(v.hi) : 0;
+    reduce<W, N, K>(v, lo, hi);
     if (MODE != WARP) {
       const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
       if (lane == 0) {
-        if (W) s.part_w[flip][warp] = v.w;
+        if (W > 0) s.part_w[flip][warp] = v.w;
+        if (W > 1) s.part_w2[flip][warp] = v.w2;
         if (N) s.part_n[flip][warp] = v.n;
         if (K) {
-          s.part_lo[flip][warp] = v.lo;
-          s.part_hi[flip][warp] = v.hi;
+          s.part_lo[flip][warp] = lo;
+          s.part_hi[flip][warp] = hi;
         }
       }
       __syncthreads();   // (two calls later the buffer is free: every thread has passed the next call's barrier)
-      v = no_sums();
-      if (lane < nw) {
-        if (W) v.w = s.part_w[flip][lane];
-        if (N) v.n = s.part_n[flip][lane];
-        if (K) {
-          v.lo = s.part_lo[flip][lane];
-          v.hi = s.part_hi[flip][lane];
-        }
+      const bool in = lane < nw;
+      if (W > 0) v.w = in ? s.part_w[flip][lane] : 0;
+      if (W > 1) v.w2 = in ? s.part_w2[flip][lane] : 0;
+      if (N) v.n = in ? s.part_n[flip][lane] : 0;
+      if (K) {
+        lo = in ? s.part_lo[flip][lane] : 0xffffffffu;
+        hi = in ? s.part_hi[flip][lane] : 0;
       }
-      reduce<W, N, K>(v);
+      reduce<W, N, K>(v, lo, hi);
       flip ^= 1;
     }
     if (MODE == CLUSTER) {
       if (threadIdx.x == 0) {
-        if (W) s.cta_w[cflip] = v.w;
+        if (W > 0) s.cta_w[cflip] = v.w;
+        if (W > 1) s.cta_w2[cflip] = v.w2;
         if (N) s.cta_n[cflip] = v.n;
         if (K) {
-          s.cta_lo[cflip] = v.lo;
-          s.cta_hi[cflip] = v.hi;
+          s.cta_lo[cflip] = lo;
+          s.cta_hi[cflip] = hi;
         }
       }
       gsync();
-      v = no_sums();
-      if (lane < (int)size) {
-        if (W) v.w = *peer(&s.cta_w[cflip], lane);
-        if (N) v.n = *peer(&s.cta_n[cflip], lane);
-        if (K) {
-          v.lo = *peer(&s.cta_lo[cflip], lane);
-          v.hi = *peer(&s.cta_hi[cflip], lane);
-        }
+      const bool in = lane < (int)size;
+      if (W > 0) v.w = in ? *peer(&s.cta_w[cflip], lane) : 0;
+      if (W > 1) v.w2 = in ? *peer(&s.cta_w2[cflip], lane) : 0;
+      if (N) v.n = in ? *peer(&s.cta_n[cflip], lane) : 0;
+      if (K) {
+        lo = in ? *peer(&s.cta_lo[cflip], lane) : 0xffffffffu;
+        hi = in ? *peer(&s.cta_hi[cflip], lane) : 0;
       }
-      reduce<W, N, K>(v);
+      reduce<W, N, K>(v, lo, hi);
       cflip ^= 1;
+    }
+    if (K) {
+      v.lo = value_of(lo);
+      v.hi = value_of(hi);
     }
     return v;
   }
-  template <bool W, bool N, bool K>
-  __device__ __forceinline__ static void reduce(Sums &v) {
-    if (W) v.w = warp_sum_u64(v.w);
+  template <int W, bool N, bool K>
+  __device__ __forceinline__ static void reduce(Sums &v, unsigned &lo, unsigned &hi) {
+    if (W > 0) v.w = warp_sum_u64(v.w);
+    if (W > 1) v.w2 = warp_sum_u64(v.w2);
     if (N) v.n = __reduce_add_sync(PK_FULL_MASK, v.n);
     if (K) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        v.lo = fminf(v.lo, __shfl_xor_sync(PK_FULL_MASK, v.lo, o));
-        v.hi = fmaxf(v.hi, __shfl_xor_sync(PK_FULL_MASK, v.hi, o));
-      }
+      lo = __reduce_min_sync(PK_FULL_MASK, lo);
+      hi = __reduce_max_sync(PK_FULL_MASK, hi);
     }
   }
 
@@ -338,8 +363,8 @@ struct Row {
   }
   // The first bin at which the bins' running sum reaches goal, `before` what the
   // bins before it hold, `inside` what it holds itself, `all` what all hold.
-  __device__ int find_bin(u64 goal, unsigned &before, unsigned &inside, u64 &all) {
-    gsync();   // every CTA's bins are filled
+  __device__ int find_bin(u64 goal, unsigned &before, unsigned &inside, u64 &all, bool synced = false) {
+    if (!synced) gsync();   // every CTA's bins are filled
     constexpr int MAXPER = MODE == WARP ? S::NB / 32 : 8;   // at least 128 threads in a CTA
     const int per = (S::NB + nt() - 1) / nt(), b0 = tid * per;
     unsigned held[MAXPER];
@@ -395,9 +420,12 @@ struct Row {
   // of them, from the largest, at which the count (BY_WEIGHT: the weight) reaches
   // `target` (1 .. what there is), given the bin that the bins of these entries
   // say. Leaves s.cut, the border's value, s.cut_take, how many of its equals
-  // belong to the prefix, s.cut_ties, how many there are.
+  // belong to the prefix, s.cut_ties, how many there are. only: the source holds
+  // the bins up to that one; false where they do not reach the target (a rounding
+  // of the hint).
   template <bool BY_WEIGHT, typename Src>
-  __device__ void border(const Src &src, float above, u64 target, int bin, unsigned bin_before, unsigned bin_inside) {
+  __device__ bool border(const Src &src, float above, u64 target, int bin, unsigned bin_before, unsigned bin_inside,
+                         bool only = false) {
     float hi = INFINITY, lo = above;          // the border is in (lo, hi], or [lo, hi] once `found`
     u64 before = bin_before;                  // count or weight of the values > hi
     unsigned inside = bin_inside;             // entries there
@@ -419,9 +447,11 @@ struct Row {
           in.w += w;
         }
       }
-      if (BY_WEIGHT) up = total<true, false, false>(up);
-      in = total<BY_WEIGHT, BY_WEIGHT, true>(in);
+      in.w2 = up.w;
+      in = total<BY_WEIGHT ? 2 : 0, BY_WEIGHT, true>(in);
+      up.w = in.w2;
       if (BY_WEIGHT) {
+        if (only && up.w + in.w < target) return false;
         found = up.w < target && target <= up.w + in.w;
         before = up.w;
         inside = in.n;
@@ -442,7 +472,7 @@ struct Row {
         in.lo = fminf(in.lo, v);
         in.hi = fmaxf(in.hi, v);
       }
-      in = total<false, true, true>(in);
+      in = total<0, true, true>(in);
       inside = in.n;
       lo = in.lo;
       hi = in.hi;
@@ -459,7 +489,7 @@ struct Row {
         up.n++;
         if (BY_WEIGHT) up.w += weight(v);
       }
-      up = total<BY_WEIGHT, true, false>(up);
+      up = total<BY_WEIGHT ? 1 : 0, true, false>(up);
       const u64 more = BY_WEIGHT ? up.w : up.n;
       if (before + more >= target) {
         lo = value_of(key_of(mid) + 1);
@@ -479,7 +509,7 @@ struct Row {
         s.cut_take = (unsigned)(BY_WEIGHT ? (target - before + each - 1) / each : target - before);
       }
       lsync();
-      return;
+      return true;
     }
     // list the candidates, in every CTA the same ones (in any order)
     if (tid == 0) s.n_cand = 0;
@@ -518,6 +548,7 @@ struct Row {
       }
     }
     gsync();   // (cluster: the candidates are read)
+    return true;
   }
 
   // The row's entries >= edge (finite) into the list, in index order, where every
@@ -596,7 +627,7 @@ struct Row {
     return true;
   }
 
-  __device__ bool small(const FromList &src, int n, long long row, int k, float p, u64 all_w, float mp, float uu);
+  __device__ bool small(int n, long long row, int k, float p, u64 all_w, float mp, float uu);
 
   // log(w / S) of a value: the exponent itself less log S, S in units of the
   // largest weight (which is one of its parts).
@@ -640,7 +671,7 @@ struct Row {
     int i = tid;
     for (; i + (G - 1) * nt() < src.n; i += G * nt()) group(i, true);
     if (i < src.n) group(i, false);
-    return total<true, false, false>(t).w;
+    return total<1, false, false>(t).w;
   }
   // The least integer that is at least p times the sum (and at least 1).
   __device__ __forceinline__ static u64 share(float p, u64 sum) {
@@ -651,7 +682,7 @@ struct Row {
     unsigned before, inside;
     u64 all;
     const u64 goal = target >> hint;
-    return find_bin(goal ? goal : 1, before, inside, all);
+    return find_bin(goal ? goal : 1, before, inside, all, MODE != WARP);   // weigh's total was a barrier
   }
   template <typename Src>
   __device__ __forceinline__ Cut top_p(const Src &src, Cut cut, float p) {
@@ -763,32 +794,33 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float
 // each step, until one entry is left in the range, or one key. False: the entries
 // weigh less than the share asked for, nothing is drawn.
 template <typename T, int MODE>
-__device__ bool Row<T, MODE>::small(const FromList &src, int n, long long row, int k, float p, u64 all_w, float mp,
+__device__ bool Row<T, MODE>::small(int n, long long row, int k, float p, u64 all_w, float mp,
                                     float uu) {
   constexpr int J = 8;
   const int lane = threadIdx.x & 31;
   unsigned key[J], wl[J], wh[J];   // key 0: dropped
-  int from[J];                     // (cluster) rank and place of the entry
   unsigned lowest = 0xffffffffu;
+  // the list (a cluster: rank and place in its list) that entry i is in
+  auto place = [&](int i, unsigned &r) {
+    r = 0;
+    if (MODE == CLUSTER)
+      for (; r < size - 1; r++) {
+        const int m = (int)*peer(&s.n_cand, r);
+        if (i < m) break;
+        i -= m;
+      }
+    return i;
+  };
 #pragma unroll
   for (int j = 0; j < J; j++) {
     const int i = 32 * j + lane;
     float v = -INFINITY;
-    from[j] = i;
+    key[j] = wl[j] = wh[j] = 0;
+    if (32 * j >= n) continue;
     if (i < n) {
-      if (MODE == CLUSTER) {
-        unsigned r = 0;
-        int at = i;
-        for (; r < size - 1; r++) {
-          const int m = (int)*peer(&s.n_cand, r);
-          if (at < m) break;
-          at -= m;
-        }
-        v = *peer(&s.list[at], r);
-        from[j] = (int)(r << 16) | at;
-      } else {
-        v = src.x[i];
-      }
+      unsigned r;
+      const int at = place(i, r);
+      v = *peer(&s.list[at], r);
     }
     const u64 w = i < n ? weight(v) : 0;
     key[j] = i < n ? key_of(v) : 0;
@@ -801,14 +833,15 @@ __device__ bool Row<T, MODE>::small(const FromList &src, int n, long long row, i
   auto count = [&](unsigned above) {
     unsigned c = 0;
 #pragma unroll
-    for (int j = 0; j < J; j++) c += key[j] > above;
+    for (int j = 0; j < J; j++)
+      if (32 * j < n) c += key[j] > above;
     return (int)__reduce_add_sync(PK_FULL_MASK, c);
   };
   auto mass = [&](unsigned above) {
     unsigned l = 0, h = 0;
 #pragma unroll
     for (int j = 0; j < J; j++)
-      if (key[j] > above) {
+      if (32 * j < n && key[j] > above) {
         l += wl[j];
         h += wh[j];
       }
@@ -890,7 +923,9 @@ __device__ bool Row<T, MODE>::small(const FromList &src, int n, long long row, i
       const u64 inc = warp_scan_u64(((u64)wh[j] << 22) + wl[j]);
       const unsigned past = __ballot_sync(PK_FULL_MASK, run + inc > target);
       if (lane == __ffs(past) - 1) {
-        a.tokens[row] = MODE == CLUSTER ? *peer(&s.index[from[j] & 0xffff], from[j] >> 16) : src.at[from[j]];
+        unsigned r;
+        const int at = place(32 * j + lane, r);
+        a.tokens[row] = *peer(&s.index[at], r);
         if (a.logprobs) a.logprobs[row] = log_prob(value_of(key[j]), sum);
       }
       break;
@@ -921,8 +956,9 @@ __device__ void Row<T, MODE>::run(long long row) {
   const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   const float uu = __ldg(a.u + row);
   // the row, once; its largest value. Its smallest finite one for the bins; a warp
-  // takes instead the smallest of its lanes' second largest: some 150 to 200
-  // entries are as large, whatever the distribution, and mostly only they matter.
+  // takes instead the smallest of its lanes' second largest: 190 +- 45 entries are as
+  // large whatever the distribution, and mostly only they matter (for the 48
+  // largest, the smallest of the lanes' largest: 130 +- 41).
   Sums v = no_sums();
   float second = -INFINITY;
 #pragma unroll 16
@@ -933,8 +969,8 @@ __device__ void Row<T, MODE>::run(long long row) {
     else v.lo = fminf(v.lo, e == -INFINITY ? INFINITY : e);
     v.hi = fmaxf(v.hi, e);
   }
-  if (MODE == WARP) v.lo = second;
-  v = total<false, false, true>(v);
+  if (MODE == WARP) v.lo = k > 0 && k <= 48 ? v.hi : second;
+  v = total<0, false, true>(v);
   if (v.hi == -INFINITY) {   // nothing to take
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
@@ -950,7 +986,7 @@ __device__ void Row<T, MODE>::run(long long row) {
       if (x[i] == v.hi) first = min(first, (unsigned)(base + i));
     Sums f = no_sums();
     f.lo = first == 0xffffffffu ? INFINITY : (float)first;   // indices below 2^18 are exact
-    f = total<false, false, true>(f);
+    f = total<0, false, true>(f);
     if (rank == 0 && tid == 0) {
       a.tokens[row] = (int)f.lo;
       if (a.logprobs) a.logprobs[row] = 0.0f;
@@ -975,13 +1011,13 @@ __device__ void Row<T, MODE>::run(long long row) {
       if (k > 0 ? k <= few.n || whole : true) {
         u64 all_w = 0;
         if (by_p && k <= 0) all_w = whole ? weigh<false>(few, -INFINITY) : weigh<false>(all, -INFINITY);
-        if (small(few, few.n, row, k, p, all_w, mp, uu)) return;
+        if (small(few.n, row, k, p, all_w, mp, uu)) return;
       }
     }
     if (k > 0 || by_p) {   // bins over the whole row
       v.lo = INFINITY;
       for (int i = tid; i < n; i += nt()) v.lo = fminf(v.lo, x[i] == -INFINITY ? INFINITY : x[i]);
-      v = total<false, false, true>(v);
+      v = total<0, false, true>(v);
     }
   }
   set_scale(fmaxf(v.lo, __fsub_rn(v.hi, 64.0f)));
@@ -990,10 +1026,10 @@ __device__ void Row<T, MODE>::run(long long row) {
     const int bin = find_bin((u64)k, before, inside, n_all);
     if ((u64)k < n_all) {
       // of a list of the bins up to the border's, or of the row
-      if (before + inside <= (unsigned)S::CAP && make_list(all, edge_of(bin), few)) {
-        if (MODE != WARP && few.total <= 256) {
+      if (MODE != WARP && before + inside <= (unsigned)S::CAP && make_list(all, edge_of(bin), few)) {
+        if (few.total <= 256) {
           gsync();   // every CTA's list is there
-          if (rank == 0 && threadIdx.x < 32) small(few, few.total, row, k, p, 0, mp, uu);
+          if (rank == 0 && threadIdx.x < 32) small(few.total, row, k, p, 0, mp, uu);
           return;
         }
         border<false>(few, -INFINITY, (u64)k, bin, before, inside);
@@ -1012,18 +1048,15 @@ __device__ void Row<T, MODE>::run(long long row) {
   if (by_p) {
     const u64 all_w = weigh<true>(all, -INFINITY), target = share(p, all_w);
     int bin = find_weight(target);
-    for (int tries = 0; tries < 2 && make_list(all, edge_of(bin), few); tries++, bin = min(bin + 1, S::NB - 1)) {
-      Sums t = no_sums();
-      for (int i = tid; i < few.n; i += nt()) {
-        const float e = few.value(i);
-        if (bin_of(e) <= bin) t.w += weight(e);
-      }
-      if (total<true, false, false>(t).w < target) continue;   // a rounding of the hint: one bin more
-      if (MODE != WARP && few.total <= 256) {
-        if (rank == 0 && threadIdx.x < 32) small(few, few.total, row, 0, p, all_w, mp, uu);
+    for (int tries = 0; MODE != WARP && tries < 2 && make_list(all, edge_of(bin), few); tries++, bin = min(bin + 1, S::NB - 1)) {
+      if (few.total <= 256) {
+        // the first CTA's first warp alone; whether the bins reach the target is a sum of few
+        const u64 have = weigh<false>(few, -INFINITY);   // (a barrier: every CTA's list is there)
+        if (have < target) continue;
+        if (rank == 0 && threadIdx.x < 32) small(few.total, row, 0, p, all_w, mp, uu);
         return;
       }
-      border<true>(few, -INFINITY, target, bin, 0, 0);
+      if (!border<true>(few, -INFINITY, target, bin, 0, 0, true)) continue;   // one bin more
       draw(few, row, read_cut(), mp, uu);
       return;
     }
@@ -1041,7 +1074,7 @@ __host__ __device__ constexpr size_t group_bytes(int seg) {
 constexpr int WARP_MAX = 2016;   // entries of a warp's row: runs of 63
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(MODE == WARP ? 256 : 1024, MODE == WARP ? 3 : 1) sample_kernel(Args a) {
+__global__ void __launch_bounds__(MODE == WARP ? 256 : 1024, MODE == WARP ? 4 : 1) sample_kernel(Args a) {
   typedef Shared<MODE> S;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double tab[16];
@@ -1077,9 +1110,9 @@ int launch(Args a, int size, int threads, cudaStream_t s) {
   const int groups = MODE == WARP ? threads / 32 : 1;
   const size_t bytes = groups * group_bytes<MODE>(a.seg);
   smem_optin(sample_kernel<T, MODE>, 200 * 1024, flags);
-  const long long most = 1 << 20;
   const long long rows = (a.n_rows + groups - 1) / groups;
   cudaLaunchConfig_t cfg = {};
+  const long long most = 1 << 20;
   cfg.gridDim = dim3((unsigned)((rows < most ? rows : most) * size));
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = bytes;
@@ -1096,20 +1129,26 @@ int launch(Args a, int size, int threads, cudaStream_t s) {
   return pkcu_launch_status("pkcu_sample_rows");
 }
 
+// Group by row length and number of rows, as measured on a B200:
+//  a warp per row for short rows where they are many: 3000 x 1025 fp32, mixed
+//  settings, 31 us against 58 with a CTA of 128 per row; 400 rows 25 against 12
+//  (a row with a wide nucleus is slow in one warp);
+//  a CTA of 128 to 1024: 100 x 1025 12.5 us with 128, 10.7 with 256; 500 x 5000 22
+//  with 256, 33 with 512; 100 x 5000 18 and 16; 256 x 32000 109 with 512, 94 with 1024;
+//  a cluster where the row does not fit a CTA's shared memory, or for few long
+//  rows: 4 x 32000 bf16, top-p, 43 us in one CTA, 30 in two, 27 in four or eight;
+//  1 x 131072 in eight CTAs of 512 33, of 1024 38; 1 x 8000 15 in one, 18 in two.
 template <typename T>
 int launch_rows(const Args &a, cudaStream_t s) {
-  static const char *e = getenv("SMODE");
-  int mode = -1, size = 1, threads = 0;
-  if (e) sscanf(e, "%d,%d,%d", &mode, &size, &threads);
-  if (mode == 0 || (mode < 0 && a.V <= WARP_MAX && a.n_rows > pkcu_sm_count())) return launch<T, WARP>(a, 1, mode < 0 ? 256 : threads, s);
-  if (mode < 0) {
-    // CTAs per row: what the logits need, and more while that leaves SMs idle
-    while ((((a.V + size - 1) / size + 31) & ~31) * 4LL > SMEM_VALUES) size *= 2;
-    while (size < 8 && a.n_rows * size * 2 <= pkcu_sm_count() && a.V / size > 4096) size *= 2;
-    const int each = (a.V + size - 1) / size;
-    threads = each <= 2048 ? 128 : each <= 8192 ? 512 : 1024;
-  }
-  return size > 1 ? launch<T, CLUSTER>(a, size, threads, s) : launch<T, CTA>(a, 1, threads, s);
+  const int sms = pkcu_sm_count();
+  if (a.V <= WARP_MAX && a.n_rows > 6LL * sms) return launch<T, WARP>(a, 1, 128, s);
+  int size = 1;
+  while ((((a.V + size - 1) / size + 31) & ~31) * 4LL > SMEM_VALUES) size *= 2;
+  while (size < 8 && a.n_rows * size * 2 <= sms && a.V / size > 8192) size *= 2;
+  const int each = (a.V + size - 1) / size;
+  if (size > 1) return launch<T, CLUSTER>(a, size, each <= 16384 ? 512 : 1024, s);
+  const int threads = each <= 512 ? 128 : each <= 2048 ? 256 : each <= 8192 ? (a.n_rows > 2 * sms ? 256 : 512) : 1024;
+  return launch<T, CTA>(a, 1, threads, s);
 }
 
 }  // namespace sample
