@@ -7,12 +7,22 @@
 // sums). The library's other products (k_tcgemm.cu) take fp32 activations as
 // three bf16 parts: three MMAs at half this rate per product.
 //
-// Orientation. The kernel computes C transposed: 128 rows of the K-major weight
-// (128 outputs n) are the MMA's M, BQ activation rows (tokens m) its N. A TMEM
-// lane then holds one n and its columns run over m, so a warp's loads and stores
-// of one token are 32 consecutive n whatever the pitch or alignment of C (rows of
-// 1025 logits included); bias and weight scale are one register per thread; and
-// one token wastes nothing but columns of a 16-wide tile.
+// Two kernels, chosen by a time model (plan() below).
+//
+// Few tokens (q8_gemm_kernel) computes C transposed: 128 rows of the K-major
+// weight (128 outputs n) are the MMA's M, 16 to 128 activation rows (tokens m) its
+// N. A TMEM lane then holds one n and its columns run over m, so a warp's loads
+// and stores of one token are 32 consecutive n whatever the pitch or alignment of
+// C (rows of 1025 logits included); bias and weight scale are one register per
+// thread; one token wastes nothing but columns of a 16-wide tile; and where the
+// tiles are few a cluster splits K. Bound by its fixed costs and the weight's
+// bytes: 1 x 1024 x 4096 5.7 us, 32 x 640 x 1025 4.7 us, 1 x 8192 x 8192 19 us =
+// 3.6 TB/s (set-up, 12 stages in flight per SM, epilogue: the products and a
+// kernel's launch alone are 3 us of the first two).
+//
+// Many tokens (q8_pair_kernel): 256 x 256 tiles of CTA pairs. 12000 x 1024 x 4096
+// int8 to bf16 51 us, with Swish 62 to 65; 12000 x 4096 x 1024 with an fp32 residual
+// 55 us; 8192^3 375 us = 2.9 Pop/s, 0.90 of twice the measured bf16 GEMM rate.
 //
 // Operands. Rows of 128 bytes of K per stage, 128-byte swizzled, by TMA (no
 // multicast); K needs no alignment: the tensor maps' extent is K itself, so
@@ -481,21 +491,21 @@ q8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   }
 }
 
-// ── many tokens: CTA pairs, rows of C by TMA ─────────────────────────────────
+// ── many tokens: CTA pairs ────────────────────────────────────────────────────
 //
-// One 256-token x BN-output tile per pair of CTAs (tcgen05 cta_group::2): each CTA
-// brings 128 tokens and half of the outputs' weight rows, the pair's MMA reads both
-// CTAs' shared memory, and each CTA's TMEM holds its 128 tokens x BN sums. So a
-// CTA loads (128 + BN / 2) bytes per byte of K for 128 x BN products: two thirds
-// of what a single CTA's 128 x 256 tile loads, which is what the L2 could not
-// deliver at the 8-bit MMA rate.
+// One 256-token x 256-output tile per pair of CTAs (tcgen05 cta_group::2): each
+// CTA brings 128 tokens and half of the outputs' weight rows, the pair's MMA reads
+// both CTAs' shared memory, and each CTA's TMEM holds its 128 tokens x 256 sums, in
+// two accumulators. So a CTA loads 256 bytes per byte of K for 128 x 256 products,
+// two thirds of what a tile of its own would (128 x 256 tiles of single CTAs moved
+// 9 to 11 TB/s from L2 and no more: 12000 x 1024 x 4096 98 us, pairs 51).
 //
-// Here a TMEM lane is a token and its columns are outputs: a thread turns 32
-// columns into 128 (or 64) consecutive bytes of its row with the scale of its
-// token in a register, writes them to a swizzled 32-row buffer of its warp with
-// 16-byte stores, and a TMA store of the box takes them to C: about 6
-// instructions per output besides the activation, against 26 for one store per
-// output and token. C must suit TMA (16-byte aligned rows).
+// Here a TMEM lane is a token and its columns are outputs: a thread turns 16
+// columns at a time into bytes of its row, with the token's scale in a register
+// and the outputs' scales and biases from shared memory, into a swizzled box of
+// its warp, which leaves as 64-byte pieces of eight rows per store: 14
+// instructions per output with Swish, against 26 for one store per output and
+// token. (A TMA store of the box measured the same and asks for aligned rows.)
 
 constexpr int CN = 16;      // columns finished at a time
 constexpr int BOX_B = 64;   // bytes of a row of a warp's box

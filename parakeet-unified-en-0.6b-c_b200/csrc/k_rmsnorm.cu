@@ -12,7 +12,11 @@
 // followed by a call without y. Both statistics come from one pass over the
 // row, so a row is read once, kept in registers as fp32, and written once: 13
 // bytes of HBM traffic per element in fp32, 7 in 16 bits. That traffic is the
-// bound.
+// bound in fp32: 12000 x 1024 in 28.0 us = 5.7 TB/s, 0.87 of the copy bandwidth,
+// 4000 x 4096 0.88. 16-bit rows take 0.8 of the time for 0.54 of the bytes (12000 x
+// 1024 bf16 22.3 us = 0.59): a row's chain of load, reduction and store is as long,
+// with half the bytes under way. Measured and not kept: persistent CTAs that load
+// the next row before they finish this one (34 to 44 us fp32, 25 to 33 bf16).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
