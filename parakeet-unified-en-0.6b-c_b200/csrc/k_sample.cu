@@ -34,6 +34,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
+#include <stdio.h>
+#include <stdlib.h>
 
 #include "pk_common.cuh"
 #include "pk_types.cuh"
@@ -188,20 +190,14 @@ __device__ __forceinline__ u64 warp_scan_u64(u64 v) {   // inclusive
   return v;
 }
 
-// Where entries come from: the row in shared memory, or the list.
-struct FromRow {
-  const float *x;
-  int n, base;
-  __device__ __forceinline__ float value(int i) const { return x[i]; }
-  __device__ __forceinline__ int index(int i) const { return base + i; }
-};
-struct FromList {
+// Where entries come from: the row in shared memory, or the list (with indices).
+struct Src {
   const float *x;
   const int *at;
-  int n;       // this CTA's
-  int total;   // the row's (not kept for a warp's)
+  int n, base;   // this CTA's number of entries
+  int total;     // a list: the row's
   __device__ __forceinline__ float value(int i) const { return x[i]; }
-  __device__ __forceinline__ int index(int i) const { return at[i]; }
+  __device__ __forceinline__ int index(int i) const { return at ? at[i] : base + i; }
 };
 
 template <typename T, int MODE>
@@ -423,7 +419,7 @@ struct Row {
   // belong to the prefix, s.cut_ties, how many there are. only: the source holds
   // the bins up to that one; false where they do not reach the target (a rounding
   // of the hint).
-  template <bool BY_WEIGHT, typename Src>
+  template <bool BY_WEIGHT>
   __device__ bool border(const Src &src, float above, u64 target, int bin, unsigned bin_before, unsigned bin_inside,
                          bool only = false) {
     float hi = INFINITY, lo = above;          // the border is in (lo, hi], or [lo, hi] once `found`
@@ -432,19 +428,27 @@ struct Row {
     bool found = !BY_WEIGHT;                  // counts need no confirmation, only the bin's values
     for (int tries = 0; tries < (BY_WEIGHT ? 3 : 1); tries++) {
       Sums up = no_sums(), in = no_sums();
-      for (int i = tid; i < src.n; i += nt()) {
-        const float v = src.value(i);
-        if (!(v > above)) continue;
-        const int b = bin_of(v);
-        if (b > bin) continue;
-        const u64 w = BY_WEIGHT ? weight(v) : 0;
-        if (b < bin) {
-          up.w += w;
-        } else {
-          in.n++;
-          in.lo = fminf(in.lo, v);
-          in.hi = fmaxf(in.hi, v);
-          in.w += w;
+      constexpr int G = BY_WEIGHT ? 6 : 4;   // independent entries side by side
+      for (int i = tid; i < src.n; i += G * nt()) {
+        float v[G];
+        u64 w[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          v[g] = i + g * nt() < src.n ? src.value(i + g * nt()) : -INFINITY;
+          w[g] = BY_WEIGHT ? weight(v[g]) : 0;
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          const int b = bin_of(v[g]);
+          if (!(v[g] > above) || b > bin) continue;
+          if (b < bin) {
+            up.w += w[g];
+          } else {
+            in.n++;
+            in.lo = fminf(in.lo, v[g]);
+            in.hi = fmaxf(in.hi, v[g]);
+            in.w += w[g];
+          }
         }
       }
       in.w2 = up.w;
@@ -553,7 +557,7 @@ struct Row {
 
   // The row's entries >= edge (finite) into the list, in index order, where every
   // CTA's fit.
-  __device__ bool make_list(const FromRow &src, float edge, FromList &out) {
+  __device__ bool make_list(const Src &src, float edge, Src &out) {
     const int lane = threadIdx.x & 31;
     edge = fmaxf(edge, -3.402823466e38f);
     if constexpr (MODE == WARP) {
@@ -624,6 +628,7 @@ struct Row {
     }
     out.x = s.list;
     out.at = s.index;
+    out.base = 0;
     return true;
   }
 
@@ -645,7 +650,7 @@ struct Row {
 
   // The sum of the weights of the values > cut; BINS: their bins too, in units of
   // which the row's total fits 32 bits.
-  template <bool BINS, typename Src>
+  template <bool BINS>
   __device__ __forceinline__ u64 weigh(const Src &src, float cut) {
     if (BINS) clear_bins();
     Sums t = no_sums();
@@ -684,27 +689,11 @@ struct Row {
     const u64 goal = target >> hint;
     return find_bin(goal ? goal : 1, before, inside, all, MODE != WARP);   // weigh's total was a barrier
   }
-  template <typename Src>
-  __device__ __forceinline__ Cut top_p(const Src &src, Cut cut, float p) {
-    const u64 w = weigh<true>(src, cut.v);
-    const u64 each = cut.ties ? weight(cut.v) : 0;
-    const u64 target = share(p, w + cut.take * each);
-    if (target > w) {   // inside the equals of the top-k's border
-      cut.take = (unsigned)((target - w + each - 1) / each);
-      return cut;
-    }
-    border<true>(src, cut.v, target, find_weight(target), 0, 0);
-    return read_cut();
-  }
-  template <typename Src>
   __device__ void draw(const Src &src, long long row, Cut cut, float mp, float uu);
-  template <typename Src>
-  __device__ __forceinline__ void count(const Src &src);
   __device__ void run(long long row);
 };
 
 template <typename T, int MODE>
-template <typename Src>
 __device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float mp, float uu) {
   const int lane = threadIdx.x & 31;
   // min-p: a weight at least min_p of the largest, which always stays
@@ -935,18 +924,6 @@ __device__ bool Row<T, MODE>::small(int n, long long row, int k, float p, u64 al
   return true;
 }
 
-// The counts of a source's entries per bin.
-template <typename T, int MODE>
-template <typename Src>
-__device__ __forceinline__ void Row<T, MODE>::count(const Src &src) {
-  clear_bins();
-#pragma unroll 8
-  for (int i = tid; i < src.n; i += nt()) {
-    const float e = src.value(i);
-    if (e > -INFINITY) atomicAdd(&s.bins[bin_of(e)], 1u);
-  }
-}
-
 template <typename T, int MODE>
 __device__ void Row<T, MODE>::run(long long row) {
   const T *in = static_cast<const T *>(a.logits) + row * a.ld + base;
@@ -956,7 +933,7 @@ __device__ void Row<T, MODE>::run(long long row) {
   const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   const float uu = __ldg(a.u + row);
   // the row, once; its largest value. Its smallest finite one for the bins; a warp
-  // takes instead the smallest of its lanes' second largest: 190 +- 45 entries are as
+  // looking for the k largest takes instead the smallest of its lanes' second largest: 190 +- 45 entries are as
   // large whatever the distribution, and mostly only they matter (for the 48
   // largest, the smallest of the lanes' largest: 130 +- 41).
   Sums v = no_sums();
@@ -969,7 +946,7 @@ __device__ void Row<T, MODE>::run(long long row) {
     else v.lo = fminf(v.lo, e == -INFINITY ? INFINITY : e);
     v.hi = fmaxf(v.hi, e);
   }
-  if (MODE == WARP) v.lo = k > 0 && k <= 48 ? v.hi : second;
+  if (MODE == WARP) v.lo = k <= 48 ? v.hi : second;
   v = total<0, false, true>(v);
   if (v.hi == -INFINITY) {   // nothing to take
     if (rank == 0 && tid == 0) {
@@ -979,7 +956,7 @@ __device__ void Row<T, MODE>::run(long long row) {
     return;
   }
   lsync();
-  const FromRow all{x, n, base};
+  const Src all{x, nullptr, n, base, 0};
   if (!(temp > 0.0f)) {   // greedy: the first largest
     unsigned first = 0xffffffffu;
     for (int i = tid; i < n; i += nt())
@@ -1001,69 +978,71 @@ __device__ void Row<T, MODE>::run(long long row) {
   }
   weight.set(v.hi, temp);
   Cut cut = {-INFINITY, 0, 0};
-  FromList few;
+  Src src = all, few;   // what is left to look at; a list
   unsigned before, inside;
   u64 n_all;
-  const bool by_p = p < 1.0f;
-  if constexpr (MODE == WARP) {
-    if ((k > 0 || by_p) && make_list(all, v.lo, few)) {
-      const bool whole = v.lo == -INFINITY;   // the list is all that can be taken
-      if (k > 0 ? k <= few.n || whole : true) {
-        u64 all_w = 0;
-        if (by_p && k <= 0) all_w = whole ? weigh<false>(few, -INFINITY) : weigh<false>(all, -INFINITY);
-        if (small(few.n, row, k, p, all_w, mp, uu)) return;
+  if (k > 0) {
+    if (MODE == WARP) {
+      // mostly the list has the k largest
+      if (make_list(all, v.lo, few) && (k <= few.n || v.lo == -INFINITY)) {
+        small(few.n, row, k, p, 0, mp, uu);
+        return;
       }
-    }
-    if (k > 0 || by_p) {   // bins over the whole row
       v.lo = INFINITY;
       for (int i = tid; i < n; i += nt()) v.lo = fminf(v.lo, x[i] == -INFINITY ? INFINITY : x[i]);
       v = total<0, false, true>(v);
     }
-  }
-  set_scale(fmaxf(v.lo, __fsub_rn(v.hi, 64.0f)));
-  if (k > 0) {
-    count(all);
+    set_scale(fmaxf(v.lo, __fsub_rn(v.hi, 64.0f)));
+    clear_bins();
+#pragma unroll 8
+    for (int i = tid; i < n; i += nt()) {
+      const float e = x[i];
+      if (e > -INFINITY) atomicAdd(&s.bins[bin_of(e)], 1u);
+    }
     const int bin = find_bin((u64)k, before, inside, n_all);
     if ((u64)k < n_all) {
-      // of a list of the bins up to the border's, or of the row
       if (MODE != WARP && before + inside <= (unsigned)S::CAP && make_list(all, edge_of(bin), few)) {
         if (few.total <= 256) {
           gsync();   // every CTA's list is there
           if (rank == 0 && threadIdx.x < 32) small(few.total, row, k, p, 0, mp, uu);
           return;
         }
-        border<false>(few, -INFINITY, (u64)k, bin, before, inside);
-        cut = read_cut();
-        if (by_p) cut = top_p(few, cut, p);
-        draw(few, row, cut, mp, uu);
-        return;
+        src = few;
       }
-      border<false>(all, -INFINITY, (u64)k, bin, before, inside);
+      border<false>(src, -INFINITY, (u64)k, bin, before, inside);
       cut = read_cut();
-      if (by_p) cut = top_p(all, cut, p);
-      draw(all, row, cut, mp, uu);
-      return;
     }
   }
-  if (by_p) {
-    const u64 all_w = weigh<true>(all, -INFINITY), target = share(p, all_w);
-    int bin = find_weight(target);
-    for (int tries = 0; MODE != WARP && tries < 2 && make_list(all, edge_of(bin), few); tries++, bin = min(bin + 1, S::NB - 1)) {
-      if (few.total <= 256) {
-        // the first CTA's first warp alone; whether the bins reach the target is a sum of few
-        const u64 have = weigh<false>(few, -INFINITY);   // (a barrier: every CTA's list is there)
-        if (have < target) continue;
-        if (rank == 0 && threadIdx.x < 32) small(few.total, row, 0, p, all_w, mp, uu);
-        return;
+  if (p < 1.0f) {
+    // below 28 T a weight is under e^-28 of the largest
+    const float low = __fsub_rn(v.hi, __fmul_rn(28.0f, temp));
+    set_scale(MODE == WARP ? low : fmaxf(v.lo, low));
+    const u64 w = weigh<true>(src, cut.v);
+    const u64 each = cut.ties ? weight(cut.v) : 0, all_w = w + cut.take * each;
+    const u64 target = share(p, all_w);
+    if (target > w) {   // inside the equals of the top-k's border
+      cut.take = (unsigned)((target - w + each - 1) / each);
+    } else {
+      int bin = find_weight(target);
+      for (int tries = cut.ties ? 2 : 0;; tries++, bin = min(bin + 1, S::NB - 1)) {
+        // of a list of the bins up to the border's; a list that proves short of the
+        // target (a rounding of the hint) is made again with one bin more
+        const bool listed = tries < 2 && make_list(all, edge_of(bin), few);
+        if (listed && MODE == WARP) {   // (the list takes the bins' place)
+          if (small(few.n, row, 0, p, all_w, mp, uu)) return;
+          tries = 2;
+        } else if (listed && few.total <= 256) {
+          if (weigh<false>(few, -INFINITY) < target) continue;   // (a barrier: every CTA's list is there)
+          if (rank == 0 && threadIdx.x < 32) small(few.total, row, 0, p, all_w, mp, uu);
+          return;
+        }
+        if (!cut.ties) src = listed && MODE != WARP ? few : all;
+        if (border<true>(src, cut.v, target, bin, 0, 0, listed && MODE != WARP)) break;
       }
-      if (!border<true>(few, -INFINITY, target, bin, 0, 0, true)) continue;   // one bin more
-      draw(few, row, read_cut(), mp, uu);
-      return;
+      cut = read_cut();
     }
-    border<true>(all, -INFINITY, target, bin, 0, 0);
-    cut = read_cut();
   }
-  draw(all, row, cut, mp, uu);
+  draw(src, row, cut, mp, uu);
 }
 
 // A group's shared memory; a warp reads up to 32 runs of odd length, and 8 more.
@@ -1071,10 +1050,13 @@ template <int MODE>
 __host__ __device__ constexpr size_t group_bytes(int seg) {
   return sizeof(Shared<MODE>) + (((size_t)(MODE == WARP ? ((seg + 31) / 32 | 1) * 32 + 8 : seg) * 4 + 15) & ~(size_t)15);
 }
+#ifndef MAXT
+#define MAXT 1024
+#endif
 constexpr int WARP_MAX = 2016;   // entries of a warp's row: runs of 63
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(MODE == WARP ? 256 : 1024, MODE == WARP ? 4 : 1) sample_kernel(Args a) {
+__global__ void __launch_bounds__(MODE == WARP ? 256 : MAXT, MODE == WARP ? 4 : 1) sample_kernel(Args a) {
   typedef Shared<MODE> S;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double tab[16];
@@ -1143,11 +1125,12 @@ int launch_rows(const Args &a, cudaStream_t s) {
   const int sms = pkcu_sm_count();
   if (a.V <= WARP_MAX && a.n_rows > 6LL * sms) return launch<T, WARP>(a, 1, 128, s);
   int size = 1;
+  if (getenv("SMODE")) { int m, sz, th; sscanf(getenv("SMODE"), "%d,%d,%d", &m, &sz, &th); if (th > MAXT) th = MAXT; return m == 0 ? launch<T, WARP>(a, 1, th, s) : sz > 1 ? launch<T, CLUSTER>(a, sz, th, s) : launch<T, CTA>(a, 1, th, s); }
   while ((((a.V + size - 1) / size + 31) & ~31) * 4LL > SMEM_VALUES) size *= 2;
   while (size < 8 && a.n_rows * size * 2 <= sms && a.V / size > 8192) size *= 2;
   const int each = (a.V + size - 1) / size;
-  if (size > 1) return launch<T, CLUSTER>(a, size, each <= 16384 ? 512 : 1024, s);
-  const int threads = each <= 512 ? 128 : each <= 2048 ? 256 : each <= 8192 ? (a.n_rows > 2 * sms ? 256 : 512) : 1024;
+  if (size > 1) return launch<T, CLUSTER>(a, size, each <= 16384 ? 512 : MAXT, s);
+  const int threads = each <= 512 ? 128 : each <= 2048 ? 256 : each <= 8192 ? (a.n_rows > 2 * sms ? 256 : 512) : MAXT;
   return launch<T, CTA>(a, 1, threads, s);
 }
 
