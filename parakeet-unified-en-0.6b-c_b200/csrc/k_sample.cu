@@ -19,23 +19,34 @@
 // 2^18 of them fits 64 bits, and it is the same in any order, so the shared
 // -memory atomics that gather candidates cannot change a result.
 //
-// Kernel. A row belongs to a group of threads: a warp (rows up to 2048 entries,
+// Kernel. A row belongs to a group of threads: a warp (rows up to 2016 entries,
 // where there are many), a CTA, or a cluster of CTAs for few long rows. Its logits
 // are read once into shared memory and everything after that works from there.
 // Top-k and top-p look for their border in a histogram of max - l over linear
-// bins (counts are exact; weights in fp32, a hint that exact sums then confirm);
-// the entries of the bins up to the border's are listed in index order and the
-// rest of the row is not looked at again. Within the border's bin the entries
-// are ranked against each other; equal logits beyond a list's length are counted
-// by halving the range of keys. For the draw each thread adds up a contiguous
+// bins (counts are exact; weights in coarse units, a hint that exact sums then
+// confirm); a warp's top-k bounds it by its lanes' largest entries instead. What is
+// as large as the border's bin is listed in index order. A list of at most 256 is
+// finished by one warp in its registers: it halves the range of keys, counting or
+// adding up weights by warp reductions, until the border is found, then draws.
+// A longer list, or the row, is looked through again by all threads: the entries of
+// the border's bin are ranked against each other (more than fit are first reduced
+// by halving the range of keys), and for the draw each thread adds up a contiguous
 // run of entries, a scan over the threads finds the run that u falls in, and the
 // run's warp finds the entry.
+//
+// What bounds it, on a B200. Not memory: 12000 x 1025 fp32 logits are 49 MB, 7.5 us
+// of reading, and take 31 us without filters (issue slots: an fp64 exponential per
+// entry and its conversions), 37 us with top-k (one per listed entry, but the list),
+// 73 us with top-p (also the bins' atomics and a second look at the row), 72 us with
+// all kinds mixed. 256 x 32000 fp32, 5 us of reading: 34 us without filters,
+// 37 with top-k, 113 with top-p, whose nuclei of thousands of entries are looked
+// through three times between barriers. 1 x 131072 bf16, in a cluster of eight: 12
+// us without filters, 17 with top-k, 32 with top-p: one cluster barrier after
+// another.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
-#include <stdio.h>
-#include <stdlib.h>
 
 #include "pk_common.cuh"
 #include "pk_types.cuh"
@@ -428,7 +439,7 @@ struct Row {
     bool found = !BY_WEIGHT;                  // counts need no confirmation, only the bin's values
     for (int tries = 0; tries < (BY_WEIGHT ? 3 : 1); tries++) {
       Sums up = no_sums(), in = no_sums();
-      constexpr int G = BY_WEIGHT ? 6 : 4;   // independent entries side by side
+      constexpr int G = MODE == WARP ? 4 : 1;   // a warp: independent entries side by side
       for (int i = tid; i < src.n; i += G * nt()) {
         float v[G];
         u64 w[G];
@@ -654,7 +665,7 @@ struct Row {
   __device__ __forceinline__ u64 weigh(const Src &src, float cut) {
     if (BINS) clear_bins();
     Sums t = no_sums();
-    constexpr int G = 6;
+    constexpr int G = 4;   // independent chains of fp64 operations; 6 fetches more code than it hides waits
     // at least the limit below which weights are 0, and past the cut
     const float low = weight.least > cut ? weight.least : cut;
     const bool past = low == cut;
@@ -714,7 +725,7 @@ __device__ void Row<T, MODE>::draw(const Src &src, long long row, Cut cut, float
   const float low0 = fmaxf(low, weight.least);   // below it weights are 0
   u64 mine = 0;
   unsigned seen = tie0;
-  constexpr int G = 6;
+  constexpr int G = 4;
   auto group = [&](int i, bool whole) {
     float v[G];
     u64 w[G];
@@ -933,12 +944,14 @@ __device__ void Row<T, MODE>::run(long long row) {
   const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   const float uu = __ldg(a.u + row);
   // the row, once; its largest value. Its smallest finite one for the bins; a warp
-  // looking for the k largest takes instead the smallest of its lanes' second largest: 190 +- 45 entries are as
-  // large whatever the distribution, and mostly only they matter (for the 48
-  // largest, the smallest of the lanes' largest: 130 +- 41).
+  // that looks for the k largest takes instead the smallest of its lanes' second
+  // largest: 190 +- 45 entries are as large whatever the distribution, and mostly
+  // only they matter (for the 48 largest, the smallest of the lanes' largest:
+  // 130 +- 41).
   Sums v = no_sums();
   float second = -INFINITY;
-#pragma unroll 16
+  constexpr int U = MODE == CTA ? 8 : 16;   // 256 x 32000 fp32 top-k 37 us with 8, 41 with 16; a warp's rows 38 and 37
+#pragma unroll U
   for (int i = tid; i < n; i += nt()) {
     const float e = clean(to_f32(in[i]));
     x[i] = e;
@@ -979,19 +992,30 @@ __device__ void Row<T, MODE>::run(long long row) {
   weight.set(v.hi, temp);
   Cut cut = {-INFINITY, 0, 0};
   Src src = all, few;   // what is left to look at; a list
-  unsigned before, inside;
-  u64 n_all;
-  if (k > 0) {
-    if (MODE == WARP) {
-      // mostly the list has the k largest
-      if (make_list(all, v.lo, few) && (k <= few.n || v.lo == -INFINITY)) {
-        small(few.n, row, k, p, 0, mp, uu);
-        return;
-      }
+  const bool by_p = p < 1.0f;
+  // a warp's few bins reach down 28 T, where a weight is e^-28 of the largest
+  const float low = __fsub_rn(v.hi, __fmul_rn(28.0f, temp));
+  u64 all_w = 0, target = 0;
+  int bin = 0;
+  if (MODE == WARP && (k > 0 || by_p)) {
+    // mostly a list of at most 256 holds all that the filters leave: with top-k, of
+    // what is as large as v.lo; without, of the bins up to the one in which p is reached
+    if (k <= 0) {
+      set_scale(low);
+      all_w = weigh<true>(all, -INFINITY);
+      target = share(p, all_w);
+      bin = find_weight(target);
+    }
+    if (make_list(all, k > 0 ? v.lo : edge_of(bin), few) && (k <= few.n || v.lo == -INFINITY) &&
+        small(few.n, row, k, p, all_w, mp, uu))
+      return;
+    if (k > 0) {
       v.lo = INFINITY;
       for (int i = tid; i < n; i += nt()) v.lo = fminf(v.lo, x[i] == -INFINITY ? INFINITY : x[i]);
       v = total<0, false, true>(v);
     }
+  }
+  if (k > 0) {
     set_scale(fmaxf(v.lo, __fsub_rn(v.hi, 64.0f)));
     clear_bins();
 #pragma unroll 8
@@ -999,9 +1023,11 @@ __device__ void Row<T, MODE>::run(long long row) {
       const float e = x[i];
       if (e > -INFINITY) atomicAdd(&s.bins[bin_of(e)], 1u);
     }
-    const int bin = find_bin((u64)k, before, inside, n_all);
-    if ((u64)k < n_all) {
-      if (MODE != WARP && before + inside <= (unsigned)S::CAP && make_list(all, edge_of(bin), few)) {
+    unsigned before, inside;
+    u64 count;
+    const int kbin = find_bin((u64)k, before, inside, count);
+    if ((u64)k < count) {
+      if (MODE != WARP && before + inside <= (unsigned)S::CAP && make_list(all, edge_of(kbin), few)) {
         if (few.total <= 256) {
           gsync();   // every CTA's list is there
           if (rank == 0 && threadIdx.x < 32) small(few.total, row, k, p, 0, mp, uu);
@@ -1009,35 +1035,34 @@ __device__ void Row<T, MODE>::run(long long row) {
         }
         src = few;
       }
-      border<false>(src, -INFINITY, (u64)k, bin, before, inside);
+      border<false>(src, -INFINITY, (u64)k, kbin, before, inside);
       cut = read_cut();
     }
   }
-  if (p < 1.0f) {
-    // below 28 T a weight is under e^-28 of the largest
-    const float low = __fsub_rn(v.hi, __fmul_rn(28.0f, temp));
-    set_scale(MODE == WARP ? low : fmaxf(v.lo, low));
-    const u64 w = weigh<true>(src, cut.v);
-    const u64 each = cut.ties ? weight(cut.v) : 0, all_w = w + cut.take * each;
-    const u64 target = share(p, all_w);
-    if (target > w) {   // inside the equals of the top-k's border
-      cut.take = (unsigned)((target - w + each - 1) / each);
-    } else {
-      int bin = find_weight(target);
+  if (by_p) {
+    bool inside_ties = false;
+    if (MODE != WARP || k > 0) {
+      set_scale(MODE == WARP ? low : fmaxf(v.lo, __fsub_rn(v.hi, 64.0f)));
+      const u64 w = weigh<true>(src, cut.v);
+      const u64 each = cut.ties ? weight(cut.v) : 0;
+      all_w = w + cut.take * each;
+      target = share(p, all_w);
+      inside_ties = target > w;   // of the top-k's border
+      if (inside_ties) cut.take = (unsigned)((target - w + each - 1) / each);
+      else bin = find_weight(target);
+    }
+    if (!inside_ties) {
       for (int tries = cut.ties ? 2 : 0;; tries++, bin = min(bin + 1, S::NB - 1)) {
         // of a list of the bins up to the border's; a list that proves short of the
         // target (a rounding of the hint) is made again with one bin more
-        const bool listed = tries < 2 && make_list(all, edge_of(bin), few);
-        if (listed && MODE == WARP) {   // (the list takes the bins' place)
-          if (small(few.n, row, 0, p, all_w, mp, uu)) return;
-          tries = 2;
-        } else if (listed && few.total <= 256) {
+        const bool listed = MODE != WARP && tries < 2 && make_list(all, edge_of(bin), few);
+        if (listed && few.total <= 256) {
           if (weigh<false>(few, -INFINITY) < target) continue;   // (a barrier: every CTA's list is there)
           if (rank == 0 && threadIdx.x < 32) small(few.total, row, 0, p, all_w, mp, uu);
           return;
         }
-        if (!cut.ties) src = listed && MODE != WARP ? few : all;
-        if (border<true>(src, cut.v, target, bin, 0, 0, listed && MODE != WARP)) break;
+        if (!cut.ties) src = listed ? few : all;
+        if (border<true>(src, cut.v, target, bin, 0, 0, listed)) break;
       }
       cut = read_cut();
     }
@@ -1050,13 +1075,10 @@ template <int MODE>
 __host__ __device__ constexpr size_t group_bytes(int seg) {
   return sizeof(Shared<MODE>) + (((size_t)(MODE == WARP ? ((seg + 31) / 32 | 1) * 32 + 8 : seg) * 4 + 15) & ~(size_t)15);
 }
-#ifndef MAXT
-#define MAXT 1024
-#endif
 constexpr int WARP_MAX = 2016;   // entries of a warp's row: runs of 63
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(MODE == WARP ? 256 : MAXT, MODE == WARP ? 4 : 1) sample_kernel(Args a) {
+__global__ void __launch_bounds__(MODE == WARP ? 256 : 1024, MODE == WARP ? 4 : 1) sample_kernel(Args a) {
   typedef Shared<MODE> S;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double tab[16];
@@ -1113,24 +1135,24 @@ int launch(Args a, int size, int threads, cudaStream_t s) {
 
 // Group by row length and number of rows, as measured on a B200:
 //  a warp per row for short rows where they are many: 3000 x 1025 fp32, mixed
-//  settings, 31 us against 58 with a CTA of 128 per row; 400 rows 25 against 12
-//  (a row with a wide nucleus is slow in one warp);
-//  a CTA of 128 to 1024: 100 x 1025 12.5 us with 128, 10.7 with 256; 500 x 5000 22
-//  with 256, 33 with 512; 100 x 5000 18 and 16; 256 x 32000 109 with 512, 94 with 1024;
+//  settings, 29 us against 50 with a CTA of 128 per row; 1000 rows 24 and 21; 400
+//  rows 22 and 12 (a row with a wide nucleus is slow in one warp);
+//  a CTA of 128 to 1024: 100 x 1025 11.5 us with 128, 10.8 with 256; 500 x 5000 23
+//  with 256, 28 with 512; 100 x 5000 18.5 and 14.8; 256 x 32000 108 with 512, 91 with
+//  1024, 94 in clusters of two of 512;
 //  a cluster where the row does not fit a CTA's shared memory, or for few long
-//  rows: 4 x 32000 bf16, top-p, 43 us in one CTA, 30 in two, 27 in four or eight;
-//  1 x 131072 in eight CTAs of 512 33, of 1024 38; 1 x 8000 15 in one, 18 in two.
+//  rows: 4 x 32000 bf16, top-p, 46 us in one CTA, 31 in two, 27 in four or eight;
+//  1 x 131072 in eight CTAs of 512 32, of 1024 34; 1 x 8000 16 in one, 21 in two.
 template <typename T>
 int launch_rows(const Args &a, cudaStream_t s) {
   const int sms = pkcu_sm_count();
   if (a.V <= WARP_MAX && a.n_rows > 6LL * sms) return launch<T, WARP>(a, 1, 128, s);
   int size = 1;
-  if (getenv("SMODE")) { int m, sz, th; sscanf(getenv("SMODE"), "%d,%d,%d", &m, &sz, &th); if (th > MAXT) th = MAXT; return m == 0 ? launch<T, WARP>(a, 1, th, s) : sz > 1 ? launch<T, CLUSTER>(a, sz, th, s) : launch<T, CTA>(a, 1, th, s); }
   while ((((a.V + size - 1) / size + 31) & ~31) * 4LL > SMEM_VALUES) size *= 2;
   while (size < 8 && a.n_rows * size * 2 <= sms && a.V / size > 8192) size *= 2;
   const int each = (a.V + size - 1) / size;
-  if (size > 1) return launch<T, CLUSTER>(a, size, each <= 16384 ? 512 : MAXT, s);
-  const int threads = each <= 512 ? 128 : each <= 2048 ? 256 : each <= 8192 ? (a.n_rows > 2 * sms ? 256 : 512) : MAXT;
+  if (size > 1) return launch<T, CLUSTER>(a, size, each <= 16384 ? 512 : 1024, s);
+  const int threads = each <= 512 ? 128 : each <= 2048 ? 256 : each <= 8192 ? (a.n_rows > 2 * sms ? 256 : 512) : 1024;
   return launch<T, CTA>(a, 1, threads, s);
 }
 
