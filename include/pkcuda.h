@@ -294,10 +294,10 @@ int pkcu_argmax_rows(const float *logits, int32_t *out, long long n_rows, int V,
  *   scales = max|n| / Q per row, Q = 127 (qtype I8) or 448 (E4M3)
  *   q      = n / scales rounded to nearest even, [n_rows, ldq] bytes (columns
  *            from D on are left as they were)
- * Arithmetic in fp32 (so entries up to about 1e18 in magnitude). x_out may be
- * x. y NULL: no residual (bias must be NULL too), the norm is of x, and x_out
- * may be NULL. bias may be NULL. A row of zeros gives q = 0 and scale 0; a row
- * with a NaN or an infinity gives q = 0 and scale NaN. ldq a multiple of 16
+ * Arithmetic in fp32. x_out may be x. y NULL: no residual (bias must be NULL
+ * too), the norm is of x, and x_out may be NULL. bias may be NULL. A row of
+ * zeros gives q = 0 and scale 0; a row with a NaN or an infinity, or whose sum
+ * of squares passes fp32's range (1024 entries of 6e17), q = 0 and scale NaN. ldq a multiple of 16
  * and q 16-byte aligned make the rows an operand of pkcu_wmatmul_q8. Pointers
  * aligned to their type; 16-byte alignment (and D a multiple of 4, of 8 in 16
  * bits) is the fast case. */
@@ -310,9 +310,9 @@ int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, f
  * the bias, the activation and the residual in the epilogue:
  *   C[m, n] = R[m, n] + rscale * act(a_scales[m] * w_scales[n] *
  *                                    sum_k A[m, k] W[k, n] + bias[n])
- * int8 x int8 summed exactly in 32-bit integers, e4m3 x e4m3 in fp32 (one
- * rounding per 32 of K at most as coarse as fp32's); the rest in fp32, rounded once to
- * C's type.
+ * int8 x int8 summed exactly in 32-bit integers, e4m3 x e4m3 in the tensor
+ * cores' fp32 accumulators (within 2^-22 of the terms' magnitudes per 32 of K);
+ * the rest in fp32, rounded once to C's type.
  * A weight is prepared once (synchronous, on the current device): data [K, N]
  * row-major device memory of type I8 (-127 .. 127 in the reference's
  * checkpoints; -128 is taken as it is) or E4M3, scales fp32 device memory, 1

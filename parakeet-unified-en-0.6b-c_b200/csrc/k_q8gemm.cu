@@ -21,7 +21,7 @@
 // kernel's launch alone are 3 us of the first two).
 //
 // Many tokens (q8_pair_kernel): 256 x 256 tiles of CTA pairs. 12000 x 1024 x 4096
-// int8 to bf16 51 us, with Swish 62 to 65; 12000 x 4096 x 1024 with an fp32 residual
+// int8 to bf16 51 us, with Swish 62 to 66; 12000 x 4096 x 1024 with an fp32 residual
 // 55 us; 8192^3 375 us = 2.9 Pop/s, 0.90 of twice the measured bf16 GEMM rate.
 //
 // Operands. Rows of 128 bytes of K per stage, 128-byte swizzled, by TMA (no
@@ -184,9 +184,11 @@ __device__ __forceinline__ void tmem_ld(unsigned taddr, unsigned (&r)[NC]) {
 
 // v / (1 + exp(-v)) on a pair: exp(-v) = 2^-h (1 + l ln 2) with h the rounded
 // product v log2 e and -l the rest of the exact one, 2^-h and the reciprocal by
-// the hardware's approximations (2 and 1 units in the last place); past 2^125
-// (v below -86) the power stands still and the result is below 1e-35.
+// the hardware's approximations (2 and 1 units in the last place). v counts as
+// -200 below that, and past 2^125 (v below -86) the power stands still: the
+// result is then within 5e-36 of 0.
 __device__ __forceinline__ float2 swish_ex2(float2 v) {
+  v = make_float2(max_nan(v.x, -200.0f), max_nan(v.y, -200.0f));
   const float2 h = mul2(v, splat2(GATE_L2E_HI));
   float2 l = fma2(v, splat2(-GATE_L2E_HI), h);
   l = mul2(fma2(v, splat2(-GATE_L2E_LO), l), splat2(0.693147180559945f));

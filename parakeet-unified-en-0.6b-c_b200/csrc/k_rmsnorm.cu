@@ -65,13 +65,6 @@ __device__ __forceinline__ float row_mul(float ss, float amax, float &up) {
   return amax == 0.0f || !row_finite(ss, amax) ? 0.0f : Quant<E4M3>::Q / (amax * up);
 }
 
-// max that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // N entries t mul rounded to nearest even, as their 8-bit patterns, for finite
 // t; |t mul| <= Q (1 + 2^-22), which rounds to Q at most, so nothing saturates.
 // int8: t mul + 1.5 2^23 in one fused multiply-add rounds to an integer whose

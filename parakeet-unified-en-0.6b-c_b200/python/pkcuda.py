@@ -272,16 +272,27 @@ def stream_handle(stream=None) -> int:
 
 # ── 8-bit activations: tensors in, one call through the C ABI ─────────────────
 
+# The checks are written for few steps: a call on one row is mostly its wrapper
+# (1 x 1024 norm: kernel 1.9 us).
+_torch = None
 _TORCH_DTYPES = {}
 
 
-def dtype_of(t) -> int:
-    """PKCU_DTYPE_* of a torch tensor."""
-    if not _TORCH_DTYPES:
+def _load_torch():
+    global _torch
+    if _torch is None:
         import torch
         _TORCH_DTYPES.update({torch.float32: PKCU_DTYPE_F32, torch.bfloat16: PKCU_DTYPE_BF16,
                               torch.float16: PKCU_DTYPE_F16, torch.int8: PKCU_DTYPE_I8,
                               torch.float8_e4m3fn: PKCU_DTYPE_E4M3})
+        _torch = torch
+    return _torch
+
+
+def dtype_of(t) -> int:
+    """PKCU_DTYPE_* of a torch tensor."""
+    if _torch is None:
+        _load_torch()
     d = _TORCH_DTYPES.get(t.dtype)
     if d is None:
         raise ValueError(f"no PKCU_DTYPE for {t.dtype}")
@@ -295,7 +306,7 @@ def _require(ok, what) -> None:
 
 def _vector(t, n, what):
     """fp32 [n], packed (or None)."""
-    if t is not None and not (dtype_of(t) == PKCU_DTYPE_F32 and t.is_contiguous() and t.numel() == n):
+    if t is not None and not (_TORCH_DTYPES.get(t.dtype) == PKCU_DTYPE_F32 and t.is_contiguous() and t.numel() == n):
         raise ValueError(f"{what}: a packed fp32 tensor of {n} entries is needed")
 
 
@@ -303,14 +314,15 @@ def _call_on(t, stream, name, *args) -> None:
     """call(name, *args, stream) on the device of t; stream: a torch stream of
     that device, None for its current one (read through torch's raw accessor:
     torch.cuda.current_stream builds an object, 3 us a call)."""
-    import torch
     dev = t.get_device()
-    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    raw = _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if dev != _torch._C._cuda_getDevice():
+        with _torch.cuda.device(dev):
             call(name, *args, raw)
     else:
-        call(name, *args, raw)
+        status = getattr(_lib or lib(), name)(*args, raw)
+        if status:
+            check(status, name)
 
 
 def _same_device(t, *others) -> None:
@@ -324,11 +336,13 @@ def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream
     """pkcu_residual_rms_norm_q8 on tensors: x, y, x_out [n_rows, D]; q [n_rows,
     >= D] int8 or float8_e4m3fn with packed columns; y, bias, x_out may be None
     as in C."""
-    _require(x.dim() == 2 and x.is_cuda and x.is_contiguous(), "x: a packed [n_rows, D] CUDA tensor is needed")
-    rows, D = x.shape
+    dtype, shape = dtype_of(x), x.shape
+    _require(len(shape) == 2 and x.is_cuda and x.is_contiguous(), "x: a packed [n_rows, D] CUDA tensor is needed")
+    rows, D = shape
     for t in (y, x_out):
-        _require(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous()),
-                 "y and x_out: the shape and type of x, packed, are needed")
+        if t is not None and t is not x:
+            _require(t.shape == shape and t.dtype == x.dtype and t.is_contiguous(),
+                     "y and x_out: the shape and type of x, packed, are needed")
     _require(q.dim() == 2 and q.shape[0] == rows and q.shape[1] >= D and (q.stride(1) == 1 or q.shape[1] == 1),
              "q: [n_rows, >= D] with packed columns is needed")
     _vector(gamma, D, "gamma")
@@ -336,7 +350,7 @@ def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream
     _vector(scales, rows, "scales")
     _same_device(x, y, bias, gamma, x_out, q, scales)
     _call_on(x, stream, "pkcu_residual_rms_norm_q8", x.data_ptr(), ptr(y), ptr(bias), alpha, gamma.data_ptr(),
-             eps, dtype_of(x), ptr(x_out), q.data_ptr(), dtype_of(q), q.stride(0) if rows > 1 else max(q.stride(0), D),
+             eps, dtype, ptr(x_out), q.data_ptr(), dtype_of(q), q.stride(0) if rows > 1 else max(q.stride(0), D),
              scales.data_ptr(), rows, D)
 
 
@@ -345,12 +359,13 @@ class WeightQ8:
     scales: a tensor of 1 or N fp32 entries, or a number."""
 
     def __init__(self, data, scales, stream=None):
-        import torch
+        torch = _load_torch()
         self.handle = VP()
         _require(data.dim() == 2 and data.is_cuda and data.is_contiguous(), "data: a packed [K, N] CUDA tensor is needed")
         K, N = data.shape
         if not torch.is_tensor(scales):
-            scales = torch.full((1,), float(scales), device=data.device)
+            with torch.cuda.stream(stream):   # None: the current one
+                scales = torch.full((1,), float(scales), device=data.device)
         _vector(scales, 1 if scales.numel() == 1 else N, "scales")
         _same_device(data, scales)
         dev = data.get_device()
@@ -387,7 +402,9 @@ def wmatmul_q8(a, a_scales, weight, out, bias=None, act=None, residual=None, rsc
     """pkcu_wmatmul_q8 on tensors: a [M, >= K] of the weight's type (its row
     pitch a multiple of 16), out and residual [M, N] with packed columns; act:
     None, "relu", "tanh", "swish" or "gelu"."""
+    dtype = dtype_of(out)
     _require(weight.handle, "the weight is closed")
+    _require(act in _ACTS, "act: None, 'relu', 'tanh', 'swish' or 'gelu' is needed")
     _require(a.dim() == 2 and a.is_cuda and a.dtype == weight.dtype and a.shape[1] >= weight.K and a.stride(1) == 1,
              "a: [M, >= K] of the weight's type with packed columns is needed")
     M = a.shape[0]
@@ -402,7 +419,7 @@ def wmatmul_q8(a, a_scales, weight, out, bias=None, act=None, residual=None, rsc
     ldc = out.stride(0) if M > 1 else max(out.stride(0), weight.N)
     ldr = 0 if residual is None else residual.stride(0) if M > 1 else max(residual.stride(0), weight.N)
     _call_on(a, stream, "pkcu_wmatmul_q8", a.data_ptr(), lda, a_scales.data_ptr(), weight.handle, ptr(bias),
-             _ACTS[act], ptr(residual), ldr, rscale, out.data_ptr(), ldc, dtype_of(out), M)
+             _ACTS[act], ptr(residual), ldr, rscale, out.data_ptr(), ldc, dtype, M)
 
 
 def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, top_p=None, min_p=None,
@@ -410,17 +427,17 @@ def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, 
     """pkcu_sample_rows on tensors: logits [n_rows, V] with packed columns,
     tokens int32 [n_rows]; temperature, top_p, min_p, u, logprobs fp32 and top_k
     int32 [n_rows] (all but u may be None)."""
-    import torch
+    dtype = dtype_of(logits)
     _require(logits.dim() == 2 and logits.is_cuda and (logits.stride(1) == 1 or logits.shape[1] == 1),
              "logits: [n_rows, V] on the GPU with packed columns is needed")
     rows, V = logits.shape
     for t in (tokens, top_k):
-        _require(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == rows),
+        _require(t is None or (t.dtype == _torch.int32 and t.is_contiguous() and t.numel() == rows),
                  "tokens and top_k: packed int32 tensors of one entry per row are needed")
     for t, what in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (logprobs, "logprobs")):
         _vector(t, rows, what)
     _same_device(logits, u, tokens, logprobs, temperature, top_k, top_p, min_p)
-    _call_on(logits, stream, "pkcu_sample_rows", logits.data_ptr(), dtype_of(logits),
+    _call_on(logits, stream, "pkcu_sample_rows", logits.data_ptr(), dtype,
              logits.stride(0) if rows > 1 else max(logits.stride(0), V), ptr(temperature), ptr(top_k), ptr(top_p),
              ptr(min_p), u.data_ptr(), tokens.data_ptr(), ptr(logprobs), rows, V)
 
