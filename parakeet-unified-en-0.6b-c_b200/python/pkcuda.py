@@ -304,17 +304,21 @@ def _require(ok, what) -> None:
         raise ValueError(what)
 
 
-def _vector(t, n, what):
-    """fp32 [n], packed (or None)."""
-    if t is not None and not (_TORCH_DTYPES.get(t.dtype) == PKCU_DTYPE_F32 and t.is_contiguous() and t.numel() == n):
-        raise ValueError(f"{what}: a packed fp32 tensor of {n} entries is needed")
+def _vector(t, n, dev, what, dtype=PKCU_DTYPE_F32):
+    """Address of a packed tensor of n entries on device dev (None for None)."""
+    if t is None:
+        return None
+    if t.numel() != n or t.get_device() != dev or not t.is_contiguous() or (
+            t.dtype is not _torch.int32 if dtype is None else _TORCH_DTYPES.get(t.dtype) != dtype):
+        raise ValueError(f"{what}: a packed {'int32' if dtype is None else 'fp32'} tensor of {n} entries on the "
+                         "device of the rows is needed")
+    return t.data_ptr()
 
 
-def _call_on(t, stream, name, *args) -> None:
-    """call(name, *args, stream) on the device of t; stream: a torch stream of
-    that device, None for its current one (read through torch's raw accessor:
+def _on(dev, stream, name, *args) -> None:
+    """call(name, *args, stream) on device dev; stream: a torch stream of that
+    device, None for its current one (read through torch's raw accessor:
     torch.cuda.current_stream builds an object, 3 us a call)."""
-    dev = t.get_device()
     raw = _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
     if dev != _torch._C._cuda_getDevice():
         with _torch.cuda.device(dev):
@@ -325,33 +329,25 @@ def _call_on(t, stream, name, *args) -> None:
             check(status, name)
 
 
-def _same_device(t, *others) -> None:
-    dev = t.get_device()
-    for o in others:
-        if o is not None and o.get_device() != dev:
-            raise ValueError("tensors on different devices")
-
-
 def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream=None) -> None:
     """pkcu_residual_rms_norm_q8 on tensors: x, y, x_out [n_rows, D]; q [n_rows,
     >= D] int8 or float8_e4m3fn with packed columns; y, bias, x_out may be None
     as in C."""
-    dtype, shape = dtype_of(x), x.shape
-    _require(len(shape) == 2 and x.is_cuda and x.is_contiguous(), "x: a packed [n_rows, D] CUDA tensor is needed")
+    dtype, shape, dev = dtype_of(x), x.shape, x.get_device()
+    if len(shape) != 2 or dev < 0 or not x.is_contiguous():
+        raise ValueError("x: a packed [n_rows, D] CUDA tensor is needed")
     rows, D = shape
     for t in (y, x_out):
-        if t is not None and t is not x:
-            _require(t.shape == shape and t.dtype == x.dtype and t.is_contiguous(),
-                     "y and x_out: the shape and type of x, packed, are needed")
-    _require(q.dim() == 2 and q.shape[0] == rows and q.shape[1] >= D and (q.stride(1) == 1 or q.shape[1] == 1),
-             "q: [n_rows, >= D] with packed columns is needed")
-    _vector(gamma, D, "gamma")
-    _vector(bias, D, "bias")
-    _vector(scales, rows, "scales")
-    _same_device(x, y, bias, gamma, x_out, q, scales)
-    _call_on(x, stream, "pkcu_residual_rms_norm_q8", x.data_ptr(), ptr(y), ptr(bias), alpha, gamma.data_ptr(),
-             eps, dtype, ptr(x_out), q.data_ptr(), dtype_of(q), q.stride(0) if rows > 1 else max(q.stride(0), D),
-             scales.data_ptr(), rows, D)
+        if t is not None and t is not x and not (
+                t.dtype is x.dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
+            raise ValueError("y and x_out: the shape, type and device of x, packed, are needed")
+    qshape, (ldq, step) = q.shape, q.stride() if q.dim() == 2 else (0, 0)
+    if len(qshape) != 2 or qshape[0] != rows or qshape[1] < D or q.get_device() != dev or (step != 1 and qshape[1] > 1):
+        raise ValueError("q: [n_rows, >= D] with packed columns on the device of x is needed")
+    _on(dev, stream, "pkcu_residual_rms_norm_q8", x.data_ptr(), None if y is None else y.data_ptr(),
+        _vector(bias, D, dev, "bias"), alpha, _vector(gamma, D, dev, "gamma"), eps, dtype,
+        None if x_out is None else x_out.data_ptr(), q.data_ptr(), dtype_of(q), ldq if rows > 1 else max(ldq, D),
+        _vector(scales, rows, dev, "scales"), rows, D)
 
 
 class WeightQ8:
@@ -366,9 +362,8 @@ class WeightQ8:
         if not torch.is_tensor(scales):
             with torch.cuda.stream(stream):   # None: the current one
                 scales = torch.full((1,), float(scales), device=data.device)
-        _vector(scales, 1 if scales.numel() == 1 else N, "scales")
-        _same_device(data, scales)
         dev = data.get_device()
+        _vector(scales, 1 if scales.numel() == 1 else N, dev, "scales")
         with torch.cuda.device(dev):
             raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
             h = VP()
@@ -402,24 +397,32 @@ def wmatmul_q8(a, a_scales, weight, out, bias=None, act=None, residual=None, rsc
     """pkcu_wmatmul_q8 on tensors: a [M, >= K] of the weight's type (its row
     pitch a multiple of 16), out and residual [M, N] with packed columns; act:
     None, "relu", "tanh", "swish" or "gelu"."""
-    dtype = dtype_of(out)
-    _require(weight.handle, "the weight is closed")
-    _require(act in _ACTS, "act: None, 'relu', 'tanh', 'swish' or 'gelu' is needed")
-    _require(a.dim() == 2 and a.is_cuda and a.dtype == weight.dtype and a.shape[1] >= weight.K and a.stride(1) == 1,
-             "a: [M, >= K] of the weight's type with packed columns is needed")
-    M = a.shape[0]
+    dtype, ashape, shape, dev = dtype_of(out), a.shape, out.shape, a.get_device()
+    N = weight.N
+    if not weight.handle:
+        raise ValueError("the weight is closed")
+    if act not in _ACTS:
+        raise ValueError("act: None, 'relu', 'tanh', 'swish' or 'gelu' is needed")
+    lda, step = a.stride() if len(ashape) == 2 else (0, 0)
+    if step != 1 or dev < 0 or a.dtype is not weight.dtype or ashape[1] < weight.K:
+        raise ValueError("a: [M, >= K] of the weight's type with packed columns is needed")
+    M = ashape[0]
+    ldc, ldr, r = 0, 0, None
     for t in (out, residual):
-        _require(t is None or (t.dim() == 2 and t.shape[0] == M and t.shape[1] == weight.N
-                               and (t.stride(1) == 1 or weight.N == 1) and t.dtype == out.dtype),
-                 "out and residual: [M, N] of one type with packed columns are needed")
-    _vector(a_scales, M, "a_scales")
-    _vector(bias, weight.N, "bias")
-    _same_device(a, a_scales, out, bias, residual)
-    lda = a.stride(0) if M > 1 else (a.shape[1] + 15) // 16 * 16
-    ldc = out.stride(0) if M > 1 else max(out.stride(0), weight.N)
-    ldr = 0 if residual is None else residual.stride(0) if M > 1 else max(residual.stride(0), weight.N)
-    _call_on(a, stream, "pkcu_wmatmul_q8", a.data_ptr(), lda, a_scales.data_ptr(), weight.handle, ptr(bias),
-             _ACTS[act], ptr(residual), ldr, rscale, out.data_ptr(), ldc, dtype, M)
+        if t is None:
+            continue
+        ldr, step = t.stride() if len(t.shape) == 2 else (0, 0)
+        if t.shape != (M, N) or t.dtype is not out.dtype or t.get_device() != dev or (step != 1 and N > 1):
+            raise ValueError("out and residual: [M, N] of one type with packed columns, on the device of a, are needed")
+        if M <= 1:
+            ldr = max(ldr, N)
+        if t is out:
+            ldc = ldr
+        if t is residual:
+            r = t.data_ptr()
+    _on(dev, stream, "pkcu_wmatmul_q8", a.data_ptr(), lda if M > 1 else (ashape[1] + 15) // 16 * 16,
+        _vector(a_scales, M, dev, "a_scales"), weight.handle, _vector(bias, N, dev, "bias"), _ACTS[act], r, ldr, rscale,
+        out.data_ptr(), ldc, dtype, M)
 
 
 def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, top_p=None, min_p=None,
@@ -427,19 +430,15 @@ def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, 
     """pkcu_sample_rows on tensors: logits [n_rows, V] with packed columns,
     tokens int32 [n_rows]; temperature, top_p, min_p, u, logprobs fp32 and top_k
     int32 [n_rows] (all but u may be None)."""
-    dtype = dtype_of(logits)
-    _require(logits.dim() == 2 and logits.is_cuda and (logits.stride(1) == 1 or logits.shape[1] == 1),
-             "logits: [n_rows, V] on the GPU with packed columns is needed")
-    rows, V = logits.shape
-    for t in (tokens, top_k):
-        _require(t is None or (t.dtype == _torch.int32 and t.is_contiguous() and t.numel() == rows),
-                 "tokens and top_k: packed int32 tensors of one entry per row are needed")
-    for t, what in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (logprobs, "logprobs")):
-        _vector(t, rows, what)
-    _same_device(logits, u, tokens, logprobs, temperature, top_k, top_p, min_p)
-    _call_on(logits, stream, "pkcu_sample_rows", logits.data_ptr(), dtype,
-             logits.stride(0) if rows > 1 else max(logits.stride(0), V), ptr(temperature), ptr(top_k), ptr(top_p),
-             ptr(min_p), u.data_ptr(), tokens.data_ptr(), ptr(logprobs), rows, V)
+    dtype, shape, dev = dtype_of(logits), logits.shape, logits.get_device()
+    ld, step = logits.stride() if len(shape) == 2 else (0, 0)
+    if len(shape) != 2 or dev < 0 or (step != 1 and shape[1] > 1):
+        raise ValueError("logits: [n_rows, V] on the GPU with packed columns is needed")
+    rows, V = shape
+    _on(dev, stream, "pkcu_sample_rows", logits.data_ptr(), dtype, ld if rows > 1 else max(ld, V),
+        _vector(temperature, rows, dev, "temperature"), _vector(top_k, rows, dev, "top_k", None),
+        _vector(top_p, rows, dev, "top_p"), _vector(min_p, rows, dev, "min_p"), _vector(u, rows, dev, "u"),
+        _vector(tokens, rows, dev, "tokens", None), _vector(logprobs, rows, dev, "logprobs"), rows, V)
 
 
 class Seq:
