@@ -14,9 +14,13 @@
 // bytes of HBM traffic per element in fp32, 7 in 16 bits. That traffic is the
 // bound in fp32: 12000 x 1024 in 28.0 us = 5.7 TB/s, 0.87 of the copy bandwidth,
 // 4000 x 4096 0.88. 16-bit rows take 0.8 of the time for 0.54 of the bytes (12000 x
-// 1024 bf16 22.3 us = 0.59): a row's chain of load, reduction and store is as long,
-// with half the bytes under way. Measured and not kept: persistent CTAs that load
-// the next row before they finish this one (34 to 44 us fp32, 25 to 33 bf16).
+// 1024 bf16 21.8 us = 0.60): 35 instructions per entry, of which the row's own part
+// (addresses, reduction, scale) is half, and gamma's and bias's fp32 reads through
+// L1 weigh twice as much. Wide 16-bit rows where they are many come through shared
+// memory by bulk copies (6000 x 8192 0.80; 1024-wide rows 24 to 28 us that way).
+// Measured and not kept: persistent CTAs that load the next row into registers
+// before they finish this one (34 to 44 us fp32, 25 to 33 bf16), rows kept packed
+// in 16 bits between the two looks at them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -26,6 +30,8 @@
 #include "pk_types.cuh"
 
 namespace pk {
+
+constexpr int RING_MAX = 8;   // rows ahead per group
 
 struct RmsArgs {
   const void *x, *y;
@@ -85,15 +91,18 @@ __device__ __forceinline__ void q8(const float *t, float mul, unsigned char *o) 
   }
 }
 
+__device__ __forceinline__ void warp_reduce(float &ss, float &amax) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(PK_FULL_MASK, ss, o);
+  // (as bits: none is negative, and NaN is above infinity)
+  amax = __uint_as_float(__reduce_max_sync(PK_FULL_MASK, __float_as_uint(amax)));
+}
+
 // (ss, amax) over the TPR threads of a row. TPR 32: the row's warp, by
 // shuffles; else the whole CTA. red: 64 floats, used once.
 template <int TPR>
 __device__ __forceinline__ void row_reduce(float &ss, float &amax, float *red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    ss += __shfl_xor_sync(PK_FULL_MASK, ss, o);
-    amax = max_nan(amax, __shfl_xor_sync(PK_FULL_MASK, amax, o));
-  }
+  warp_reduce(ss, amax);
   if (TPR > 32) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int W = TPR / 32;
@@ -266,6 +275,126 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rms_q8_kernel(RmsArgs a
   if (t == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
 }
 
+// ── many rows in 16 bits ──────────────────────────────────────────────────────
+// One CTA per SM, of G groups of TPR threads. A group takes rows first, first +
+// step, ... through a ring of its own: bulk copies bring x and y of the next rows
+// into shared memory while this one is worked on, so bytes under way need no
+// registers and no thread waits for the whole of a row's latency; gamma and bias
+// stay in registers. A slot is free once the row's reduction has passed its
+// barrier (every thread holds its entries by then).
+template <typename T, bool E4M3, int TPR, int NV, int G>
+__global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int stages) {
+  constexpr int VEC = 16 / (int)sizeof(T), W = TPR / 32;
+  extern __shared__ __align__(128) unsigned char ring_smem[];
+  __shared__ unsigned long long full[G][RING_MAX];
+  __shared__ float red[2][G][2][W];   // the row's partial sums and maxima; alternating
+  __shared__ int stop[G];
+  const int g = threadIdx.x / TPR, t = threadIdx.x % TPR, lane = t & 31, warp = t >> 5;
+  const int nc = a.D / VEC;
+  const unsigned row_bytes = (unsigned)a.D * sizeof(T), slot = a.y ? 2 * row_bytes : row_bytes;
+  unsigned char *ring = ring_smem + (size_t)g * stages * slot;
+  const long long first = (long long)blockIdx.x * G + g, step = (long long)gridDim.x * G;
+  auto load = [&](long long row, int i) {
+    mbar_arrive_tx(&full[g][i], slot);
+    bulk_g2s(ring + i * slot, static_cast<const T *>(a.x) + row * a.D, row_bytes, &full[g][i]);
+    if (a.y) bulk_g2s(ring + i * slot + row_bytes, static_cast<const T *>(a.y) + row * a.D, row_bytes, &full[g][i]);
+  };
+  if (t == 0) {
+    for (int i = 0; i < stages; i++) mbar_init(&full[g][i], 1);
+    mbar_init_fence();
+    stop[g] = 0;
+    for (int i = 0; i < stages; i++)
+      if (first + i * step < a.n_rows) load(first + i * step, i);
+  }
+  float gm[NV][VEC], bs[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+    if (t + j * TPR < nc) {
+      load_param<VEC>(gm[j], a.gamma + (t + j * TPR) * VEC);
+      if (a.bias) load_param<VEC>(bs[j], a.bias + (t + j * TPR) * VEC);
+    }
+  __syncthreads();
+  int at = 0, phase = 0, flip = 0;
+  for (long long row = first; row < a.n_rows; row += step) {
+    const bool here = mbar_wait(&full[g][at], phase);
+    if (!here) {
+      if (t == 0) atomicAdd(&g_wait_timeouts, 1u);
+      stop[g] = 1;
+    }
+    const Pack<T, VEC> *sx = reinterpret_cast<const Pack<T, VEC> *>(ring + at * slot);
+    const Pack<T, VEC> *sy = reinterpret_cast<const Pack<T, VEC> *>(ring + at * slot + row_bytes);
+    Pack<T, VEC> px[NV];   // x'
+    float ss = 0.0f, amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if (t + j * TPR < nc) {
+        px[j] = sx[t + j * TPR];
+        if (a.y) {
+          const Pack<T, VEC> py = sy[t + j * TPR];
+#pragma unroll
+          for (int i = 0; i < VEC; i++) {
+            float add = to_f32(py.e[i]);
+            if (a.bias) add = add + bs[j][i];
+            px[j].e[i] = from_f32<T>(fmaf(add, a.alpha, to_f32(px[j].e[i])));
+          }
+        }
+        if (a.x_out && here)
+          reinterpret_cast<Pack<T, VEC> *>(static_cast<T *>(a.x_out) + row * a.D)[t + j * TPR] = px[j];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          const float x1 = to_f32(px[j].e[i]);
+          ss = fmaf(x1, x1, ss);
+          amax = max_nan(amax, fabsf(x1 * gm[j][i]));
+        }
+      }
+    warp_reduce(ss, amax);
+    if (lane == 0) {
+      red[flip][g][0][warp] = ss;
+      red[flip][g][1][warp] = amax;
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(TPR) : "memory");
+    if (*(volatile int *)&stop[g]) break;
+    if (t == 0 && row + stages * step < a.n_rows) load(row + stages * step, at);
+    ss = red[flip][g][0][0];
+    amax = red[flip][g][1][0];
+#pragma unroll
+    for (int w = 1; w < W; w++) {
+      ss += red[flip][g][0][w];
+      amax = max_nan(amax, red[flip][g][1][w]);
+    }
+    float up;
+    const float mul = row_mul<E4M3>(ss, amax, up);
+    unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if (t + j * TPR < nc) {
+        Pack<unsigned char, VEC> o = {};
+        float n[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) n[i] = to_f32(px[j].e[i]) * gm[j][i];
+        if (up != 1.0f) {
+#pragma unroll
+          for (int i = 0; i < VEC; i++) n[i] *= up;
+        }
+        if (mul != 0.0f) q8<E4M3, VEC>(n, mul, o.e);
+        *reinterpret_cast<Pack<unsigned char, VEC> *>(q + (t + j * TPR) * VEC) = o;
+      }
+    if (t == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
+    flip ^= 1;
+    if (++at == stages) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+  // a wait ran out: the copies still in flight land (bounded) before the CTA's
+  // shared memory is released
+  if (t == 0 && *(volatile int *)&stop[g])
+    for (int i = 0; i < stages; i++) {
+      mbar_wait(&full[g][i], 0);
+      mbar_wait(&full[g][i], 1);
+    }
+}
+
 template <typename T, bool E4M3, int VEC, int TPR, int EPT>
 void rms_launch_as(const RmsArgs &a, cudaStream_t s) {
   const long long grid = TPR == 32 ? (a.n_rows + 7) / 8 : a.n_rows;
@@ -278,6 +407,22 @@ void rms_launch_as(const RmsArgs &a, cudaStream_t s) {
 // flight per SM). Wider rows take 16 or 32 per thread: 4000 x 4096 fp32 35.8 us
 // with 256 of 16, 36.9 with 512 of 8; 2049 x 8192 fp32 37.9 with 512 of 16, 39.9
 // with 256 of 32, but bf16, whose chunks take half the registers, 35.8 and 32.8.
+// Many wide 16-bit rows go through the ring: 2049 x 8192 bf16 32.8 us in registers,
+// 27.7 through the ring, 6000 x 8192 75.8 and 65.5, 4000 x 5120 42.0 and 36.8; 900 x
+// 8192 16.8 and 17.2 (too few rows per group); up to 4096 wide the two are within
+// 10 % of each other, and the registers win below 3000 rows.
+constexpr int RING_BYTES = 200 * 1024;
+template <typename T, bool E4M3, int TPR, int NV, int G>
+void rms_launch_ring(const RmsArgs &a, cudaStream_t s) {
+  static int flags[64];
+  smem_optin(rms_q8_ring_kernel<T, E4M3, TPR, NV, G>, RING_BYTES, flags);
+  const int slot = a.D * (int)sizeof(T) * (a.y ? 2 : 1);
+  const int fit = RING_BYTES / (G * slot), stages = fit < RING_MAX ? fit : RING_MAX;
+  const long long ctas = (a.n_rows + G - 1) / G;
+  const int sms = pkcu_sm_count();
+  rms_q8_ring_kernel<T, E4M3, TPR, NV, G><<<(unsigned)(ctas < sms ? ctas : sms), TPR * G, (size_t)stages * G * slot, s>>>(a, stages);
+}
+
 template <typename T, bool E4M3, int VEC>
 void rms_launch_rows(const RmsArgs &a, cudaStream_t s) {
   if (a.D <= 256) rms_launch_as<T, E4M3, VEC, 32, 8>(a, s);
@@ -285,8 +430,10 @@ void rms_launch_rows(const RmsArgs &a, cudaStream_t s) {
   else if (a.D <= 1024) rms_launch_as<T, E4M3, VEC, 128, 8>(a, s);
   else if (a.D <= 2048) rms_launch_as<T, E4M3, VEC, 256, 8>(a, s);
   else if (a.D <= 4096) rms_launch_as<T, E4M3, VEC, 256, 16>(a, s);
-  else if (VEC == 8) rms_launch_as<T, E4M3, VEC, 256, 32>(a, s);
-  else rms_launch_as<T, E4M3, VEC, 512, 16>(a, s);
+  else if constexpr (VEC == 8) {
+    if (a.n_rows >= 8LL * pkcu_sm_count()) rms_launch_ring<T, E4M3, 256, 4, 2>(a, s);
+    else rms_launch_as<T, E4M3, VEC, 256, 32>(a, s);
+  } else rms_launch_as<T, E4M3, VEC, 512, 16>(a, s);
 }
 
 template <typename T, bool E4M3>
@@ -308,6 +455,8 @@ int rms_launch(const RmsArgs &a, int e4m3, cudaStream_t s) {
 }  // namespace pk
 
 using namespace pk;
+
+PK_WAIT_TIMEOUTS_ACCESSOR(pk_rms_wait_timeouts)
 
 extern "C" int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, float alpha,
                                          const float *gamma, float eps, int dtype, void *x_out, void *q,

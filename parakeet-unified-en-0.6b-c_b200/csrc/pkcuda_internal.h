@@ -55,6 +55,7 @@ int pk_conv_wait_timeouts(unsigned *count, int reset);
 int pk_tc_wait_timeouts(unsigned *count, int reset);   /* k_tcgemm.cu */
 
 int pk_q8_wait_timeouts(unsigned *count, int reset);   /* k_q8gemm.cu */
+int pk_rms_wait_timeouts(unsigned *count, int reset);  /* k_rmsnorm.cu */
 /* The driver's cuTensorMapEncodeTiled (looked up once, k_tcgemm.cu). */
 int pk_tensor_map_encoder(void **fn);
 

@@ -159,3 +159,57 @@ def test_stream_and_graph(cuda):
 def test_no_rows(cuda):
     cuda.call("pkcu_residual_rms_norm_q8", None, None, None, 1.0, None, EPS, 0, None, None, 1, 1024, None, 0, 1024,
               None)
+
+
+@pytest.mark.parametrize("q", ["i8", "e4m3"])
+@pytest.mark.parametrize("rows,D,dtype,parts", [(1184, 4104, "bf16", "yb"), (1185, 8192, "f16", "y"), (2400, 5000, "bf16", ""),
+                                                (1700, 8184, "bf16", "y"), (1300, 8192, "f32", "yb")])
+def test_many_wide_rows(cuda, rows, D, dtype, parts, q):
+    """In place, rows of NaN, of infinity and of zeros among the others, what
+    lies behind a row left as it was; twice the same bits, and from a graph."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(rows + D)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    x = (2 * n(rows, D)).to(torch_dtype(dtype))
+    x[5], x[rows - 1] = 0.0, 0.0
+    x[7, D - 1], x[rows - 2, 0], x[9] = float("nan"), float("inf"), 1e-4
+    y = n(rows, D).to(x.dtype) if parts else None
+    if parts:
+        y[5], y[rows - 1] = 0.0, 0.0
+    bias = 0.1 * n(D) if "b" in parts else None
+    gamma = 1 + 0.2 * n(D)
+    outs = []
+    for _ in range(2):
+        xo = x.clone()
+        outs.append(run(cuda, xo, y, bias, 0.5, gamma, q, pitch=D + 16 - D % 8, x_out=xo if parts else None))
+    xo, qt, scales = outs[0]
+    view = lambda t: t.view(torch.uint8)
+    assert torch.equal(view(qt), view(outs[1][1])) and torch.equal(scales.view(torch.int32), outs[1][2].view(torch.int32))
+    stored = xo if parts else x
+    if parts:
+        add = y.double() if bias is None else y.double() + bias.double()
+        want = x.double() + 0.5 * add
+        tol = HALF_STEP[dtype] * want.abs() + 2 * U * (want.abs() + x.double().abs()) + 2.0 ** -25 * (dtype == "f16")
+        fine = torch.isfinite(want)
+        assert ((stored.double() - want).abs()[fine] <= tol[fine]).all()
+    odd = ~torch.isfinite(stored.double()).all(dim=1)
+    assert odd.nonzero().flatten().tolist() == [7, rows - 2]
+    s = f64(scales)
+    assert np.isnan(s[[7, rows - 2]]).all() and (view(qt)[[7, rows - 2], :D] == 0).all()
+    if bias is None:
+        assert s[5] == 0 and s[rows - 1] == 0 and (view(qt)[5, :D] == 0).all()
+    assert (view(qt)[:, D:] == 0x55).all()
+    # rows of all parts of the run, among them the last of every group
+    some = sorted(({0, 1, 5, 9, rows - 1, rows - 3} | set(range(11, rows, 37)) | set(range(rows - 300, rows - 2, 7))) - {7})
+    if bias is None:
+        some = [i for i in some if i not in (5, rows - 1)]
+    check(f64(stored[some]), f64(gamma), f64(qt[some][:, :D].float()), s[some], q)
+    q2, s2 = empty(qt.shape, torch.uint8).fill_(0x55).view(qt.dtype), empty(rows)
+    xi, xg = torch.zeros_like(x), torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cuda.residual_rms_norm_q8(xi, y, bias, 0.5, gamma, EPS, xg if parts else None, q2, s2)
+    xi.copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(view(q2), view(qt)) and torch.equal(s2.view(torch.int32), scales.view(torch.int32))
