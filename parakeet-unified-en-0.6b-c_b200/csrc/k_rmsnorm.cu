@@ -32,6 +32,7 @@
 namespace pk {
 
 constexpr int RING_MAX = 8;   // rows ahead per group
+constexpr int LONG_THREADS = 1024;
 
 struct RmsArgs {
   const void *x, *y;
@@ -122,41 +123,6 @@ __device__ __forceinline__ void row_reduce(float &ss, float &amax, float *red) {
   }
 }
 
-// ── any row length: one CTA per row, two passes (the second from x_out) ───────
-
-template <typename T, bool E4M3>
-__global__ void __launch_bounds__(256) rms_q8_long_kernel(RmsArgs a) {
-  __shared__ float red[64];
-  const long long row = blockIdx.x;
-  const T *x = static_cast<const T *>(a.x) + row * a.D;
-  const T *y = a.y ? static_cast<const T *>(a.y) + row * a.D : nullptr;
-  T *xo = a.x_out ? static_cast<T *>(a.x_out) + row * a.D : nullptr;
-  float ss = 0.0f, amax = 0.0f;
-  for (int i = threadIdx.x; i < a.D; i += 256) {
-    float v = to_f32(x[i]);
-    if (y) {
-      float t = to_f32(y[i]);
-      if (a.bias) t = t + __ldg(a.bias + i);
-      v = to_f32(from_f32<T>(fmaf(t, a.alpha, v)));
-    }
-    if (xo) xo[i] = from_f32<T>(v);
-    ss = fmaf(v, v, ss);
-    amax = max_nan(amax, fabsf(v * __ldg(a.gamma + i)));
-  }
-  row_reduce<256>(ss, amax, red);
-  float up;
-  const float mul = row_mul<E4M3>(ss, amax, up);
-  unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
-  const T *v = xo ? xo : x;   // each thread re-reads the entries that it wrote itself
-  for (int i = threadIdx.x; i < a.D; i += 256) {
-    const float t = to_f32(v[i]) * __ldg(a.gamma + i) * up;
-    unsigned char o = 0;
-    if (mul != 0.0f) q8<E4M3, 1>(&t, mul, &o);
-    q[i] = o;
-  }
-  if (threadIdx.x == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
-}
-
 // ── rows held in registers ────────────────────────────────────────────────────
 // TPR threads per row (a warp, eight rows to a CTA; or a whole CTA), each
 // holding EPT entries in chunks of VEC (16 bytes of the stream's type, or one
@@ -198,6 +164,59 @@ __device__ __forceinline__ void load_param(float (&o)[VEC], const float *p) {
   }
 }
 
+// ── any row length: one CTA per row, two passes (the second from x_out) ───────
+template <typename T, bool E4M3, int VEC>
+__global__ void __launch_bounds__(LONG_THREADS) rms_q8_long_kernel(RmsArgs a) {
+  __shared__ float red[64];
+  const long long row = blockIdx.x;
+  const int nc = a.D / VEC;
+  const T *x = static_cast<const T *>(a.x) + row * a.D;
+  const T *y = a.y ? static_cast<const T *>(a.y) + row * a.D : nullptr;
+  T *xo = a.x_out ? static_cast<T *>(a.x_out) + row * a.D : nullptr;
+  float ss = 0.0f, amax = 0.0f;
+#pragma unroll 2
+  for (int c = threadIdx.x; c < nc; c += LONG_THREADS) {
+    Pack<T, VEC> px = load_pack<T, VEC, false>(x + (long long)c * VEC);
+    float p[VEC];
+    if (y) {
+      const Pack<T, VEC> py = load_pack<T, VEC, true>(y + (long long)c * VEC);
+      if (a.bias) load_param<VEC>(p, a.bias + (long long)c * VEC);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        float add = to_f32(py.e[i]);
+        if (a.bias) add = add + p[i];
+        px.e[i] = from_f32<T>(fmaf(add, a.alpha, to_f32(px.e[i])));
+      }
+    }
+    if (xo) *reinterpret_cast<Pack<T, VEC> *>(xo + (long long)c * VEC) = px;
+    load_param<VEC>(p, a.gamma + (long long)c * VEC);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      const float v = to_f32(px.e[i]);
+      ss = fmaf(v, v, ss);
+      amax = max_nan(amax, fabsf(v * p[i]));
+    }
+  }
+  row_reduce<LONG_THREADS>(ss, amax, red);
+  float up;
+  const float mul = row_mul<E4M3>(ss, amax, up);
+  unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
+  const T *v = xo ? xo : x;   // each thread re-reads the entries that it wrote itself
+#pragma unroll 2
+  for (int c = threadIdx.x; c < nc; c += LONG_THREADS) {
+    const Pack<T, VEC> px = load_pack<T, VEC, false>(v + (long long)c * VEC);
+    float n[VEC];
+    load_param<VEC>(n, a.gamma + (long long)c * VEC);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) n[i] = to_f32(px.e[i]) * n[i] * up;
+    Pack<unsigned char, VEC> o = {};
+    if (mul != 0.0f) q8<E4M3, VEC>(n, mul, o.e);
+    *reinterpret_cast<Pack<unsigned char, VEC> *>(q + (long long)c * VEC) = o;
+  }
+  if (threadIdx.x == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
+}
+
+// ── rows held in registers: the kernel ────────────────────────────────────────
 template <typename T, bool E4M3, int TPR, int VEC, int EPT>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rms_q8_kernel(RmsArgs a) {
   constexpr int NV = EPT / VEC, ROWS = TPR == 32 ? 8 : 1;
@@ -441,7 +460,8 @@ int rms_launch_q(const RmsArgs &a, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.x_out | (uintptr_t)a.bias | (uintptr_t)a.gamma;
   const bool vec = a.D % VEC == 0 && (at & 15) == 0 && ((uintptr_t)a.q | (uintptr_t)a.ldq) % VEC == 0;
-  if (a.D > 8192) rms_q8_long_kernel<T, E4M3><<<(unsigned)a.n_rows, 256, 0, s>>>(a);
+  if (a.D > 8192 && vec) rms_q8_long_kernel<T, E4M3, VEC><<<(unsigned)a.n_rows, LONG_THREADS, 0, s>>>(a);
+  else if (a.D > 8192) rms_q8_long_kernel<T, E4M3, 1><<<(unsigned)a.n_rows, LONG_THREADS, 0, s>>>(a);
   else if (vec) rms_launch_rows<T, E4M3, VEC>(a, s);
   else rms_launch_rows<T, E4M3, 1>(a, s);
   return pkcu_launch_status("pkcu_residual_rms_norm_q8");

@@ -213,3 +213,17 @@ def test_many_wide_rows(cuda, rows, D, dtype, parts, q):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(view(q2), view(qt)) and torch.equal(s2.view(torch.int32), scales.view(torch.int32))
+
+
+@pytest.mark.parametrize("D,offset", [(9001, 0), (16384, 0), (16384, 1), (20008, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_rows_in_place(cuda, dtype, D, offset):
+    r = np.random.default_rng(D)
+    x, y = (cu(r.standard_normal((5, D)).astype(np.float32), dtype, offset) for _ in range(2))
+    gamma = cu((1 + 0.2 * r.standard_normal(D)).astype(np.float32))
+    before = f64(x)
+    run(cuda, x, y, None, 1.0, gamma, "i8", x_out=x)
+    want = before + f64(y)
+    assert (np.abs(f64(x) - want) <= (HALF_STEP[dtype] + 2 * U) * np.abs(want) + U * np.abs(before)).all()
+    x, q, s = x, *run(cuda, x, None, None, 0.0, gamma, "e4m3")[1:]
+    check(f64(x), f64(gamma), f64(q), f64(s), "e4m3")
