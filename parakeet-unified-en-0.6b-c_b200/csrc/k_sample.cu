@@ -35,14 +35,15 @@
 // run's warp finds the entry.
 //
 // What bounds it, on a B200. Not memory: 12000 x 1025 fp32 logits are 49 MB, 7.5 us
-// of reading, and take 31 us without filters (issue slots: an fp64 exponential per
-// entry and its conversions), 37 us with top-k (one per listed entry, but the list),
-// 73 us with top-p (also the bins' atomics and a second look at the row), 72 us with
-// all kinds mixed. 256 x 32000 fp32, 5 us of reading: 34 us without filters,
-// 37 with top-k, 113 with top-p, whose nuclei of thousands of entries are looked
-// through three times between barriers. 1 x 131072 bf16, in a cluster of eight: 12
-// us without filters, 17 with top-k, 32 with top-p: one cluster barrier after
-// another.
+// of reading, and take 30 us without filters (issue slots: 62 instructions per entry,
+// of which the fp64 exponential and its conversions are 40), 37 us with top-k (one per
+// listed entry, but the list), 74 us with top-p (also the bins' atomics and a second
+// look at the row), 73 us with all kinds mixed. 256 x 32000 fp32, 5 us of reading: 28
+// us without filters, 32 with top-k, 104 with top-p, whose nuclei of thousands of
+// entries are looked through three times between barriers. 1 x 131072 bf16, in a
+// cluster of eight: 11 us without filters, 17 with top-k, 32 with top-p: one cluster
+// barrier after another. Not kept: contiguous runs per thread in every pass with the
+// draw's sums taken from top-p's (the same), more loads in flight per thread (more registers).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -83,18 +84,24 @@ __device__ __forceinline__ float value_of(unsigned k) {
   return __uint_as_float(k ^ (~(unsigned)((int)k >> 31) | 0x80000000u));
 }
 
-// 2^(i / 16)
+// e^x on |x| <= ln 2 / 32 by the Taylor series of degree 5 (the next term is below
+// 1.5e-13), with x = r L, L = ln 2 / 16, as K (((((r + a) r + b) r + c) r + d) r + e),
+// K = L^5 / 120, a = 5 / L, b = 20 / L^2, c = 60 / L^3, d = 120 / L^4, e = 120 / L^5:
+// one constant per operation, each read from constant memory as an operand (as
+// literals they took more instructions than the arithmetic). kPow2: K 2^44 2^(i / 16).
+__constant__ double kExp[5] = {115.41560327111708, 10656.609182748713, 737963.386590881, 34068995.78215325, 786418740.2076721};
 __constant__ double kPow2[16] = {
-    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484,
-    1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407,
-    1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+    22369.998507118962, 23360.40295392472, 24394.656351723497, 25474.700059431234,
+    26602.56138726612, 27780.35740213786, 29010.298901515907, 30294.694563235866,
+    31635.955279033526, 33036.59867994085, 34499.25386203834, 36026.66632143434,
+    37621.70310773456, 39287.35820567516, 41026.758155021096, 42843.167919278625};
+// Sums that round to an integer: 1.5 2^52 and 2^52.
+__constant__ double kRound[2] = {6755399441055744.0, 4503599627370496.0};
 
 // exp((v - max) / T) as an integer multiple of 2^-44, rounded; 2^44 for v = max
 // (finite). With y = (v - max) 16 log2(e) / T = n + r, |r| <= 1/2: 2^(y / 16) =
-// 2^(n div 16) 2^((n mod 16) / 16) e^(r ln 2 / 16), the last by the Taylor series
-// of degree 5 (|r ln 2 / 16| < 0.0217: the next term is below 1.5e-13). Sums that
-// round to an integer are formed by adding 1.5 2^52. Below `least`, where the
-// weight is under 2^-60, the result is 0 whatever the arithmetic gives.
+// 2^(n div 16) 2^((n mod 16) / 16) e^(r L). Below `least`, where the weight is under
+// 2^-60, the result is 0 whatever the arithmetic gives.
 struct Weight {
   const double *tab;   // kPow2 in shared memory
   double c, top;       // 16 log2(e) / T; max
@@ -108,18 +115,18 @@ struct Weight {
   // For v >= least (else any number).
   __device__ __forceinline__ u64 raw(float v) const {
     const double d = __dadd_rn((double)v, -top);
-    constexpr double kShift = 6755399441055744.0;   // 1.5 2^52
-    const double t = fma(d, c, kShift);
-    const double r = fma(d, c, -__dadd_rn(t, -kShift));
+    const double t = fma(d, c, kRound[0]);
+    const double r = fma(d, c, __dadd_rn(kRound[0], -t));
     const int n = __double2loint(t);
-    constexpr double L = 0.693147180559945309417 / 16;
-    const double r2 = __dmul_rn(r, r);
-    double p = fma(fma(r, L * L * L * L * L / 120, L * L * L * L / 24), r2, fma(r, L * L * L / 6, L * L / 2));
-    p = fma(p, r2, fma(r, L, 1.0));
+    double p = __dadd_rn(r, kExp[0]);
+    p = fma(p, r, kExp[1]);
+    p = fma(p, r, kExp[2]);
+    p = fma(p, r, kExp[3]);
+    p = fma(p, r, kExp[4]);
     const double w = __dmul_rn(tab[n & 15], p);
-    // times 2^(n div 16 + 44), then to an integer: the mantissa after adding 2^52
-    const double s = __hiloint2double(__double2hiint(w) + (((n >> 4) + 44) << 20), __double2loint(w));
-    return (u64)__double_as_longlong(__dadd_rn(s, 4503599627370496.0)) - 0x4330000000000000ull;
+    // times 2^(n div 16), then to an integer: the mantissa after adding 2^52
+    const double s = __hiloint2double(__double2hiint(w) + ((n & ~15) << 16), __double2loint(w));
+    return (u64)__double_as_longlong(__dadd_rn(s, kRound[1])) - 0x4330000000000000ull;
   }
   __device__ __forceinline__ u64 operator()(float v) const { return v >= least ? raw(v) : 0; }
   // (v - max) / T
@@ -162,7 +169,7 @@ struct Both<WARP> {
   };
 };
 template <int MODE>
-struct Shared : Both<MODE> {
+struct alignas(16) Shared : Both<MODE> {
   static constexpr int NB = Binned<MODE>::NB, CAP = Listed<MODE>::CAP, RANK = Binned<MODE>::RANK;
   static constexpr int NW = MODE == WARP ? 1 : 32;
   u64 part_w[2][NW], part_w2[2][NW];   // a warp's part of a reduction or scan; alternating
@@ -216,7 +223,7 @@ struct Row {
   typedef Shared<MODE> S;
   const Args &a;
   S &s;
-  float *x;             // this group's (CTA's) entries
+  float *room, *x;      // this group's (CTA's) entries, in room from where their alignment asks
   int base, n;          // the first one's index in the row, their number
   unsigned rank, size;  // of the cluster
   int tid;              // thread of the group (CTA)
@@ -950,14 +957,39 @@ __device__ void Row<T, MODE>::run(long long row) {
   // 130 +- 41).
   Sums v = no_sums();
   float second = -INFINITY;
-  constexpr int U = MODE == CTA ? 8 : 16;   // 256 x 32000 fp32 top-k 37 us with 8, 41 with 16; a warp's rows 38 and 37
-#pragma unroll U
-  for (int i = tid; i < n; i += nt()) {
-    const float e = clean(to_f32(in[i]));
-    x[i] = e;
+  auto take = [&](float e) {
     if (MODE == WARP) second = fmaxf(second, fminf(v.hi, e));
     else v.lo = fminf(v.lo, e == -INFINITY ? INFINITY : e);
     v.hi = fmaxf(v.hi, e);
+  };
+  // 16 bytes at a time from the first 16-byte boundary on, which shared memory has at
+  // the same place, what lies before it and behind the last whole piece singly: 256 x
+  // 32000 fp32 top-k 37 us by single entries, 32 by pieces, 12000 x 100 42 and 35 (12000
+  // x 1025, whose rows are aligned to their type alone, 36 and 36.6)
+  constexpr int E = 16 / (int)sizeof(T);
+  const int mis = (int)((uintptr_t)in / sizeof(T)) & (E - 1);
+  x = room + mis;
+  const int lo = min((E - mis) & (E - 1), n), pieces = (n - lo) / E, hi = lo + pieces * E;
+  const int edge = tid < lo ? tid : tid + (hi - lo);   // fewer than 2 E: one per thread
+  T at_edge = from_f32<T>(0.0f);
+  if (edge < n) at_edge = in[edge];
+#pragma unroll 4
+  for (int c = tid; c < pieces; c += nt()) {
+    const uint4 q = *reinterpret_cast<const uint4 *>(in + lo + c * E);
+    const T *e = reinterpret_cast<const T *>(&q);
+    float f[E];
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+      f[j] = clean(to_f32(e[j]));
+      take(f[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < E; j += 4) *reinterpret_cast<float4 *>(x + lo + c * E + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+  }
+  if (edge < n) {
+    const float e = clean(to_f32(at_edge));
+    x[edge] = e;
+    take(e);
   }
   if (MODE == WARP) v.lo = k <= 48 ? v.hi : second;
   v = total<0, false, true>(v);
@@ -1070,10 +1102,11 @@ __device__ void Row<T, MODE>::run(long long row) {
   draw(src, row, cut, mp, uu);
 }
 
-// A group's shared memory; a warp reads up to 32 runs of odd length, and 8 more.
+// A group's shared memory: entries from up to 7 places on; a warp reads up to 32 runs
+// of odd length, and 8 more.
 template <int MODE>
 __host__ __device__ constexpr size_t group_bytes(int seg) {
-  return sizeof(Shared<MODE>) + (((size_t)(MODE == WARP ? ((seg + 31) / 32 | 1) * 32 + 8 : seg) * 4 + 15) & ~(size_t)15);
+  return sizeof(Shared<MODE>) + (((size_t)((MODE == WARP ? ((seg + 31) / 32 | 1) * 32 + 8 : seg) + 7) * 4 + 15) & ~(size_t)15);
 }
 constexpr int WARP_MAX = 2016;   // entries of a warp's row: runs of 63
 
@@ -1089,7 +1122,7 @@ __global__ void __launch_bounds__(MODE == WARP ? 256 : 1024, MODE == WARP ? 4 : 
   unsigned char *mem = smem + (MODE == WARP ? warp * group : 0);
   S &s = *reinterpret_cast<S *>(mem);
   Row<T, MODE> r{a, s};
-  r.x = reinterpret_cast<float *>(mem + sizeof(S));
+  r.x = r.room = reinterpret_cast<float *>(mem + sizeof(S));
   r.hint = 44 - 31 + (32 - __clz(a.V));   // V < 2^(32 - clz) weights of 2^44: 31 bits
   r.weight.tab = tab;
   r.flip = r.cflip = 0;

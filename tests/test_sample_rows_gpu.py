@@ -215,3 +215,16 @@ def test_greedy_is_the_argmax(cuda):
     cuda.call("pkcu_argmax_rows", x.data_ptr(), a.data_ptr(), 500, 1025, cuda.stream_handle())
     cuda.sample_rows(x, torch.rand(500, device="cuda"), t, temperature=torch.zeros(500, device="cuda"))
     assert torch.equal(a, t)
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 5), ("f32", 1027), ("bf16", 9), ("bf16", 1030), ("bf16", 2016), ("f16", 2017),
+                                     ("bf16", 40001)])
+def test_rows_of_every_alignment(cuda, dtype, V):
+    """A pitch of one entry more than a multiple of 16 bytes: rows start at every
+    place that their type allows; enough of them for a warp per row where V allows."""
+    rng = np.random.default_rng(V)
+    rows = 1500 if V < 5000 else 20
+    pitch = (V + 7) // 8 * 8 + 1
+    wide = cu((3 * rng.standard_normal((rows, pitch))).astype(np.float32), dtype, 1)
+    wide[:, V:] = 50.0   # never a row's
+    check(cuda, wide[:, :V], rng.random(rows).astype(np.float32), **settings(rng, rows, "mixed"))
