@@ -39,8 +39,8 @@
 // of which the fp64 exponential and its conversions are 40), 37 us with top-k (one per
 // listed entry, but the list), 74 us with top-p (also the bins' atomics and a second
 // look at the row), 73 us with all kinds mixed. 256 x 32000 fp32, 5 us of reading: 28
-// us without filters, 32 with top-k, 104 with top-p, whose nuclei of thousands of
-// entries are looked through three times between barriers. 1 x 131072 bf16, in a
+// us without filters, 32 with top-k, 76 with top-p, whose nuclei of thousands of
+// entries are looked through three or four times between barriers. 1 x 131072 bf16, in a
 // cluster of eight: 11 us without filters, 17 with top-k, 32 with top-p: one cluster
 // barrier after another. Not kept: contiguous runs per thread in every pass with the
 // draw's sums taken from top-p's (the same), more loads in flight per thread (more registers).
@@ -701,11 +701,12 @@ struct Row {
     const u64 t = p > 0.0f ? (u64)ceil((double)p * (double)sum) : 1;
     return t < 1 ? 1 : t < sum ? t : sum;
   }
-  __device__ __forceinline__ int find_weight(u64 target) {
+  __device__ __forceinline__ int find_weight(u64 target, u64 &binned) {   // binned: what the bins hold
     unsigned before, inside;
-    u64 all;
     const u64 goal = target >> hint;
-    return find_bin(goal ? goal : 1, before, inside, all, MODE != WARP);   // weigh's total was a barrier
+    const int bin = find_bin(goal ? goal : 1, before, inside, binned, MODE != WARP);   // weigh's total was a barrier
+    binned <<= hint;
+    return bin;
   }
   __device__ void draw(const Src &src, long long row, Cut cut, float mp, float uu);
   __device__ void run(long long row);
@@ -1036,7 +1037,8 @@ __device__ void Row<T, MODE>::run(long long row) {
       set_scale(low);
       all_w = weigh<true>(all, -INFINITY);
       target = share(p, all_w);
-      bin = find_weight(target);
+      u64 binned;
+      bin = find_weight(target, binned);
     }
     if (make_list(all, k > 0 ? v.lo : edge_of(bin), few) && (k <= few.n || v.lo == -INFINITY) &&
         small(few.n, row, k, p, all_w, mp, uu))
@@ -1081,7 +1083,23 @@ __device__ void Row<T, MODE>::run(long long row) {
       target = share(p, all_w);
       inside_ties = target > w;   // of the top-k's border
       if (inside_ties) cut.take = (unsigned)((target - w + each - 1) / each);
-      else bin = find_weight(target);
+      else {
+        u64 binned;
+        bin = find_weight(target, binned);
+        // weights below half a unit are missing from the bins: where that is more than
+        // 2^-8 of the sum and the border is among weights of a few units, again in finer
+        // units, now that the sum is known (1 x 131072 bf16, top-p 0.98: 59 us, 163
+        // without, the border's bin being far off; top-p 0.6, where it is not needed, 31
+        // us, 41 if it were always done)
+        const int coarse = hint, fine = 33 - __clzll((long long)w);   // w < 2^31 fine units
+        if (MODE != WARP && fine < coarse && binned + (w >> 8) < w && weight(edge_of(bin)) < (4ull << coarse)) {
+          hint = max(fine, 0);
+          gsync();   // (cluster: the bins are read)
+          weigh<true>(src, cut.v);
+          bin = find_weight(target, binned);
+          hint = coarse;
+        }
+      }
     }
     if (!inside_ties) {
       for (int tries = cut.ties ? 2 : 0;; tries++, bin = min(bin + 1, S::NB - 1)) {

@@ -228,3 +228,16 @@ def test_rows_of_every_alignment(cuda, dtype, V):
     wide = cu((3 * rng.standard_normal((rows, pitch))).astype(np.float32), dtype, 1)
     wide[:, V:] = 50.0   # never a row's
     check(cuda, wide[:, :V], rng.random(rows).astype(np.float32), **settings(rng, rows, "mixed"))
+
+
+@pytest.mark.parametrize("rows,V", [(6, 32000), (2, 131072), (160, 20000)])
+def test_wide_nuclei(cuda, rows, V):
+    """Nuclei of most of the row, whose entries weigh little each; after a top-k too."""
+    rng = np.random.default_rng(V)
+    x = (2.5 * rng.standard_normal((rows, V))).astype(np.float32)
+    x[::2, rng.integers(0, V, 4)] += 9.0
+    u = rng.random(rows).astype(np.float32)
+    p = np.resize(np.array([0.9, 0.97, 0.99, 0.999, 0.9999, 0.5], np.float32), rows)
+    for dtype in ("f32", "bf16"):
+        check(cuda, cu(x, dtype), u, p=p, T=np.full(rows, 1.1), what="top-p")
+        check(cuda, cu(x, dtype), u, p=p, k=np.full(rows, V // 3), what="both")
