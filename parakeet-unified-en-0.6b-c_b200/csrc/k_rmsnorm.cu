@@ -12,15 +12,15 @@
 // followed by a call without y. Both statistics come from one pass over the
 // row, so a row is read once, kept in registers as fp32, and written once: 13
 // bytes of HBM traffic per element in fp32, 7 in 16 bits. That traffic is the
-// bound in fp32: 12000 x 1024 in 28.0 us = 5.7 TB/s, 0.87 of the copy bandwidth,
-// 4000 x 4096 0.88. 16-bit rows take 0.8 of the time for 0.54 of the bytes (12000 x
-// 1024 bf16 21.8 us = 0.60): 35 instructions per entry, of which the row's own part
-// (addresses, reduction, scale) is half, and gamma's and bias's fp32 reads through
-// L1 weigh twice as much. Wide 16-bit rows where they are many come through shared
-// memory by bulk copies (6000 x 8192 0.80; 1024-wide rows 24 to 28 us that way).
-// Measured and not kept: persistent CTAs that load the next row into registers
-// before they finish this one (34 to 44 us fp32, 25 to 33 bf16), rows kept packed
-// in 16 bits between the two looks at them.
+// bound in fp32: 12000 x 1024 to int8 in 28.0 us = 5.7 TB/s, 0.87 of the copy
+// bandwidth, to e4m3 28.7; 4000 x 4096 0.88. 16-bit rows take 0.8 of the time for 0.54
+// of the bytes (12000 x 1024 bf16 22.4 us = 0.59): 35 instructions per entry, of which
+// the row's own part (addresses, reduction, scale) is half, and gamma's and bias's fp32
+// reads through L1 weigh twice as much. Wide 16-bit rows where they are many come
+// through shared memory by bulk copies (2049 x 8192 to int8 0.70 without a bias, 6000 x
+// 8192 0.80; 1024-wide rows 24 to 28 us that way). Measured and not kept: persistent
+// CTAs that load the next row into registers before they finish this one (34 to 44 us
+// fp32, 25 to 33 bf16), rows kept packed in 16 bits between the two looks at them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -65,30 +65,67 @@ __device__ __forceinline__ float row_scale(float ss, float amax, float eps, int 
   const float r = 1.0f / sqrtf(ss / (float)D + eps);
   return amax * r / Quant<E4M3>::Q;
 }
-// Q / max|t|, 0 for a row whose q is 0; up: what t is multiplied by first.
+// Q / max|t| (max|t| times up, what t is multiplied by first), 0 for a row whose q
+// is 0; lo (e4m3): what its rounding left.
+struct RowMul {
+  float hi, lo, up;
+};
 template <bool E4M3>
-__device__ __forceinline__ float row_mul(float ss, float amax, float &up) {
-  up = amax < kTiny ? kTinyUp : 1.0f;
-  return amax == 0.0f || !row_finite(ss, amax) ? 0.0f : Quant<E4M3>::Q / (amax * up);
+__device__ __forceinline__ RowMul row_mul(float ss, float amax) {
+  RowMul m;
+  m.up = amax < kTiny ? kTinyUp : 1.0f;
+  m.hi = amax == 0.0f || !row_finite(ss, amax) ? 0.0f : Quant<E4M3>::Q / (amax * m.up);
+  m.lo = E4M3 ? fmaf(-m.hi, amax * m.up, Quant<E4M3>::Q) * (m.hi * (1.0f / Quant<E4M3>::Q)) : 0.0f;
+  return m;
 }
 
-// N entries t mul rounded to nearest even, as their 8-bit patterns, for finite
-// t; |t mul| <= Q (1 + 2^-22), which rounds to Q at most, so nothing saturates.
-// int8: t mul + 1.5 2^23 in one fused multiply-add rounds to an integer whose
-// two's complement is the sum's low byte.
+// N entries x gamma mul rounded to nearest even, as their 8-bit patterns, for
+// finite ones; |x gamma mul| <= Q (1 + 2^-22), which rounds to Q at most, so
+// nothing saturates. int8: t = x gamma, and t mul + 1.5 2^23 in one fused
+// multiply-add rounds to an integer whose two's complement is the sum's low byte.
+// e4m3: what the two products and mul itself lost is added before the rounding, so
+// that entries next to a border between two values fall on the side of the exact
+// ones (half as many of them astray as the plain product leaves).
 template <bool E4M3, int N>
-__device__ __forceinline__ void q8(const float *t, float mul, unsigned char *o) {
+__device__ __forceinline__ void q8(const float (&x)[N], const float (&g)[N], RowMul m, unsigned char *o) {
+  float v[N];
+  if constexpr (E4M3) {   // two entries per operation; c: the correction, negative
+    const float2 neg = splat2(-1.0f), hi = splat2(m.hi), nhi = splat2(-m.hi), nlo = splat2(-m.lo);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 x2 = make_float2(x[i], N > 1 ? x[i + (N > 1)] : 0.0f), g2 = make_float2(g[i], N > 1 ? g[i + (N > 1)] : 0.0f);
+      float2 t = mul2(x2, g2), lo = fma2(x2, g2, mul2(t, neg));
+      if (m.up != 1.0f) {
+        t = mul2(t, splat2(m.up));
+        lo = mul2(lo, splat2(m.up));
+      }
+      const float2 p = mul2(t, hi);
+      const float2 c = fma2(lo, nhi, fma2(t, nlo, fma2(t, nhi, p)));
+      const float2 r = fma2(c, neg, p);
+      v[i] = r.x;
+      if (N > 1) v[i + (N > 1)] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = x[i] * g[i];
+    if (m.up != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] *= m.up;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = fmaf(v[i], m.hi, 12582912.0f);
+  }
   if constexpr (E4M3) {
 #pragma unroll
     for (int i = 0; i + 1 < N; i += 2) {
-      const __nv_fp8x2_storage_t p = __nv_cvt_float2_to_fp8x2(make_float2(t[i] * mul, t[i + 1] * mul), __NV_SATFINITE, __NV_E4M3);
+      const __nv_fp8x2_storage_t p = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
       o[i] = (unsigned char)(p & 0xff);
       o[i + 1] = (unsigned char)(p >> 8);
     }
-    if (N & 1) o[N - 1] = __nv_cvt_float_to_fp8(t[N - 1] * mul, __NV_SATFINITE, __NV_E4M3);
+    if (N & 1) o[N - 1] = __nv_cvt_float_to_fp8(v[N - 1], __NV_SATFINITE, __NV_E4M3);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) o[i] = (unsigned char)(__float_as_uint(fmaf(t[i], mul, 12582912.0f)) & 0xff);
+    for (int i = 0; i < N; i++) o[i] = (unsigned char)(__float_as_uint(v[i]) & 0xff);
   }
 }
 
@@ -198,19 +235,18 @@ __global__ void __launch_bounds__(LONG_THREADS) rms_q8_long_kernel(RmsArgs a) {
     }
   }
   row_reduce<LONG_THREADS>(ss, amax, red);
-  float up;
-  const float mul = row_mul<E4M3>(ss, amax, up);
+  const RowMul mul = row_mul<E4M3>(ss, amax);
   unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
-  const T *v = xo ? xo : x;   // each thread re-reads the entries that it wrote itself
+  const T *kept = xo ? xo : x;   // each thread re-reads the entries that it wrote itself
 #pragma unroll 2
   for (int c = threadIdx.x; c < nc; c += LONG_THREADS) {
-    const Pack<T, VEC> px = load_pack<T, VEC, false>(v + (long long)c * VEC);
-    float n[VEC];
-    load_param<VEC>(n, a.gamma + (long long)c * VEC);
+    const Pack<T, VEC> px = load_pack<T, VEC, false>(kept + (long long)c * VEC);
+    float v[VEC], g[VEC];
+    load_param<VEC>(g, a.gamma + (long long)c * VEC);
 #pragma unroll
-    for (int i = 0; i < VEC; i++) n[i] = to_f32(px.e[i]) * n[i] * up;
+    for (int i = 0; i < VEC; i++) v[i] = to_f32(px.e[i]);
     Pack<unsigned char, VEC> o = {};
-    if (mul != 0.0f) q8<E4M3, VEC>(n, mul, o.e);
+    if (mul.hi != 0.0f) q8<E4M3, VEC>(v, g, mul, o.e);
     *reinterpret_cast<Pack<unsigned char, VEC> *>(q + (long long)c * VEC) = o;
   }
   if (threadIdx.x == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
@@ -270,25 +306,27 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rms_q8_kernel(RmsArgs a
       load_param<VEC>(g, a.gamma + (t + j * TPR) * VEC);
 #pragma unroll
       for (int i = 0; i < VEC; i++) {
-        const float x1 = v[j * VEC + i];
+        const float x1 = v[j * VEC + i], n = x1 * g[i];
         ss = fmaf(x1, x1, ss);
-        v[j * VEC + i] = x1 * g[i];
-        amax = max_nan(amax, fabsf(v[j * VEC + i]));
+        amax = max_nan(amax, fabsf(n));
+        if (!E4M3) v[j * VEC + i] = n;
       }
     }
   row_reduce<TPR>(ss, amax, red);
-  float up;
-  const float mul = row_mul<E4M3>(ss, amax, up);
-  if (up != 1.0f) {
-#pragma unroll
-    for (int i = 0; i < EPT; i++) v[i] *= up;
-  }
+  const RowMul mul = row_mul<E4M3>(ss, amax);
   unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
 #pragma unroll
   for (int j = 0; j < NV; j++)
     if (t + j * TPR < nc) {
       Pack<unsigned char, VEC> o = {};
-      if (mul != 0.0f) q8<E4M3, VEC>(v + j * VEC, mul, o.e);
+      float x1[VEC], g[VEC];   // e4m3: gamma once more; int8: x gamma is at hand
+      if (E4M3) load_param<VEC>(g, a.gamma + (t + j * TPR) * VEC);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        x1[i] = v[j * VEC + i];
+        if (!E4M3) g[i] = 1.0f;
+      }
+      if (mul.hi != 0.0f) q8<E4M3, VEC>(x1, g, mul, o.e);
       *reinterpret_cast<Pack<unsigned char, VEC> *>(q + (t + j * TPR) * VEC) = o;
     }
   if (t == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
@@ -298,8 +336,9 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rms_q8_kernel(RmsArgs a
 // One CTA per SM, of G groups of TPR threads. A group takes rows first, first +
 // step, ... through a ring of its own: bulk copies bring x and y of the next rows
 // into shared memory while this one is worked on, so bytes under way need no
-// registers and no thread waits for the whole of a row's latency; gamma and bias
-// stay in registers. A slot is free once the row's reduction has passed its
+// registers and no thread waits for the whole of a row's latency; gamma and
+// bias stay in registers (bias read again from L1 for every row: 2049 x 8192 to int8
+// 31.7 us for 27.6). A slot is free once the row's reduction has passed its
 // barrier (every thread holds its entries by then).
 template <typename T, bool E4M3, int TPR, int NV, int G>
 __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int stages) {
@@ -381,21 +420,16 @@ __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int s
       ss += red[flip][g][0][w];
       amax = max_nan(amax, red[flip][g][1][w]);
     }
-    float up;
-    const float mul = row_mul<E4M3>(ss, amax, up);
+    const RowMul mul = row_mul<E4M3>(ss, amax);
     unsigned char *q = static_cast<unsigned char *>(a.q) + row * a.ldq;
 #pragma unroll
     for (int j = 0; j < NV; j++)
       if (t + j * TPR < nc) {
         Pack<unsigned char, VEC> o = {};
-        float n[VEC];
+        float v[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) n[i] = to_f32(px[j].e[i]) * gm[j][i];
-        if (up != 1.0f) {
-#pragma unroll
-          for (int i = 0; i < VEC; i++) n[i] *= up;
-        }
-        if (mul != 0.0f) q8<E4M3, VEC>(n, mul, o.e);
+        for (int i = 0; i < VEC; i++) v[i] = to_f32(px[j].e[i]);
+        if (mul.hi != 0.0f) q8<E4M3, VEC>(v, gm[j], mul, o.e);
         *reinterpret_cast<Pack<unsigned char, VEC> *>(q + (t + j * TPR) * VEC) = o;
       }
     if (t == 0) a.scales[row] = row_scale<E4M3>(ss, amax, a.eps, a.D);
@@ -426,10 +460,10 @@ void rms_launch_as(const RmsArgs &a, cudaStream_t s) {
 // flight per SM). Wider rows take 16 or 32 per thread: 4000 x 4096 fp32 35.8 us
 // with 256 of 16, 36.9 with 512 of 8; 2049 x 8192 fp32 37.9 with 512 of 16, 39.9
 // with 256 of 32, but bf16, whose chunks take half the registers, 35.8 and 32.8.
-// Many wide 16-bit rows go through the ring: 2049 x 8192 bf16 32.8 us in registers,
-// 27.7 through the ring, 6000 x 8192 75.8 and 65.5, 4000 x 5120 42.0 and 36.8; 900 x
-// 8192 16.8 and 17.2 (too few rows per group); up to 4096 wide the two are within
-// 10 % of each other, and the registers win below 3000 rows.
+// Many wide 16-bit rows go through the ring: 2049 x 8192 bf16 to int8 31.7 us in
+// registers, 27.6 through the ring, to e4m3 36.8 and 31.6; 6000 x 8192 76 and 65; 4000 x
+// 5120 42 and 37; 900 x 8192 16.8 and 17.2 (too few rows per group). Up to 4096 wide the
+// two are within 10 % of each other, and the registers win below 3000 rows.
 constexpr int RING_BYTES = 200 * 1024;
 template <typename T, bool E4M3, int TPR, int NV, int G>
 void rms_launch_ring(const RmsArgs &a, cudaStream_t s) {
