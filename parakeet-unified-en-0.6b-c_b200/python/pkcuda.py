@@ -274,14 +274,15 @@ def stream_handle(stream=None) -> int:
 
 # The checks are written for few steps: a call on one row is mostly its wrapper
 # (1 x 1024 norm: kernel 1.9 us).
-_torch = None
+_torch = _F32 = _I32 = None
 _TORCH_DTYPES = {}
 
 
 def _load_torch():
-    global _torch
+    global _torch, _F32, _I32
     if _torch is None:
         import torch
+        _F32, _I32 = torch.float32, torch.int32
         _TORCH_DTYPES.update({torch.float32: PKCU_DTYPE_F32, torch.bfloat16: PKCU_DTYPE_BF16,
                               torch.float16: PKCU_DTYPE_F16, torch.int8: PKCU_DTYPE_I8,
                               torch.float8_e4m3fn: PKCU_DTYPE_E4M3})
@@ -304,14 +305,21 @@ def _require(ok, what) -> None:
         raise ValueError(what)
 
 
-def _vector(t, n, dev, what, dtype=PKCU_DTYPE_F32):
-    """Address of a packed tensor of n entries on device dev (None for None)."""
+def _vector(t, n, dev, what):
+    """Address of a packed fp32 tensor of n entries on device dev (None for None)."""
     if t is None:
         return None
-    if t.numel() != n or t.get_device() != dev or not t.is_contiguous() or (
-            t.dtype is not _torch.int32 if dtype is None else _TORCH_DTYPES.get(t.dtype) != dtype):
-        raise ValueError(f"{what}: a packed {'int32' if dtype is None else 'fp32'} tensor of {n} entries on the "
-                         "device of the rows is needed")
+    if t.dtype is not _F32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: a packed fp32 tensor of {n} entries on the device of the rows is needed")
+    return t.data_ptr()
+
+
+def _ints(t, n, dev, what):
+    """The same of an int32 tensor."""
+    if t is None:
+        return None
+    if t.dtype is not _I32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: a packed int32 tensor of {n} entries on the device of the rows is needed")
     return t.data_ptr()
 
 
@@ -436,9 +444,9 @@ def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, 
         raise ValueError("logits: [n_rows, V] on the GPU with packed columns is needed")
     rows, V = shape
     _on(dev, stream, "pkcu_sample_rows", logits.data_ptr(), dtype, ld if rows > 1 else max(ld, V),
-        _vector(temperature, rows, dev, "temperature"), _vector(top_k, rows, dev, "top_k", None),
+        _vector(temperature, rows, dev, "temperature"), _ints(top_k, rows, dev, "top_k"),
         _vector(top_p, rows, dev, "top_p"), _vector(min_p, rows, dev, "min_p"), _vector(u, rows, dev, "u"),
-        _vector(tokens, rows, dev, "tokens", None), _vector(logprobs, rows, dev, "logprobs"), rows, V)
+        _ints(tokens, rows, dev, "tokens"), _vector(logprobs, rows, dev, "logprobs"), rows, V)
 
 
 class Seq:
