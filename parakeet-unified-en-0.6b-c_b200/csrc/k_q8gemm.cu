@@ -576,17 +576,6 @@ __device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // TMEM columns without waiting; tmem_wait() before the first use.
-__device__ __forceinline__ void tmem_ld_async(unsigned taddr, unsigned (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_ld_async(unsigned taddr, unsigned (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
@@ -595,17 +584,6 @@ __device__ __forceinline__ void tmem_ld_async(unsigned taddr, unsigned (&r)[16])
       : "r"(taddr));
 }
 // The registers pass through, so that no use moves above the wait.
-__device__ __forceinline__ void tmem_wait(unsigned (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
-
 __device__ __forceinline__ void tmem_wait(unsigned (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
@@ -613,7 +591,7 @@ __device__ __forceinline__ void tmem_wait(unsigned (&r)[16]) {
                : "memory");
 }
 
-// 32 entries n .. n + 31 of a row of R as raw 16-byte words (r NULL: none).
+// CN entries n .. n + CN - 1 of a row of R as raw 16-byte words (r NULL: none).
 template <typename T>
 struct RowChunk {
   static constexpr int VEC = 16 / (int)sizeof(T);
@@ -631,7 +609,7 @@ struct RowChunk {
   }
 };
 
-// 32 sums of this thread's token with scales and bias. par: for each pair of
+// CN sums of this thread's token with scales and bias. par: for each pair of
 // outputs the two scales and the two biases, in shared memory, the same for
 // every lane.
 template <bool E4M3>
@@ -847,7 +825,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       }
       if (!ok) continue;
       tc_fence_after();
-      // 32 columns at a time; the next ones' TMEM load is in flight while the
+      // CN columns at a time; the next ones' TMEM load is in flight while the
       // activation and the store of these go on, and their residual after it
       unsigned acc[CN];
       const unsigned t0 = tmem + lane_addr + buf * BN;
