@@ -254,7 +254,12 @@ def reference_arm(args, rank, world):
     """--impl reference: rank 0 times the reference CPU implementation."""
     if rank != 0:
         return
-    r = RefRunner(args.T, args.blocks)
+    try:
+        r = RefRunner(args.T, args.blocks)
+    except FileNotFoundError:
+        print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref/libpkref.so not built (reference tree absent)"}),
+              flush=True)
+        return
     for _ in range(args.warmup):
         r.run_one()
     t0 = time.perf_counter()
@@ -1375,12 +1380,16 @@ def _ours(args, rank, world, local_rank, stream):
         print(json.dumps({"extras": run_extras(args, stream, world)}), flush=True)
     cpu = None
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
-        r = RefRunner(args.T, args.blocks)
-        fps, n_utts, secs = r.sample(args.cpu_seconds)
-        cpu = {"value": fps, "unit": "frames/s", "cores": r.threads, "kind": "reference",
-               "sample": f"{n_utts} utterance(s) x T={args.T} x {args.blocks} blocks through the "
-                         f"reference's own conformer_block (GEMMs as no-ops), "
-                         f"PK_THREADS={r.threads}, {secs:.1f} s"}
+        try:
+            r = RefRunner(args.T, args.blocks)
+        except FileNotFoundError:
+            cpu = {"unavailable": "oracle/_ref/libpkref.so not built"}
+        else:
+            fps, n_utts, secs = r.sample(args.cpu_seconds)
+            cpu = {"value": fps, "unit": "frames/s", "cores": r.threads, "kind": "reference",
+                   "sample": f"{n_utts} utterance(s) x T={args.T} x {args.blocks} blocks through the "
+                             f"reference's own conformer_block (GEMMs as no-ops), "
+                             f"PK_THREADS={r.threads}, {secs:.1f} s"}
     if rank != 0:
         return
     peak, peak_kind = measured_peak()
