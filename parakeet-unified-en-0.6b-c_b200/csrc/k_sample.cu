@@ -376,7 +376,9 @@ struct Row {
     lsync();
   }
   // The first bin at which the bins' running sum reaches goal, `before` what the
-  // bins before it hold, `inside` what it holds itself, `all` what all hold.
+  // bins before it hold, `inside` what it holds itself, `all` what all hold. It ends
+  // with a barrier of this CTA alone: a peer may still read this CTA's bins, so they
+  // are not filled again before a barrier of the cluster.
   __device__ int find_bin(u64 goal, unsigned &before, unsigned &inside, u64 &all, bool synced = false) {
     if (!synced) gsync();   // every CTA's bins are filled
     constexpr int MAXPER = MODE == WARP ? S::NB / 32 : 8;   // at least 128 threads in a CTA
@@ -1071,6 +1073,8 @@ __device__ void Row<T, MODE>::run(long long row) {
       }
       border<false>(src, -INFINITY, (u64)k, kbin, before, inside);
       cut = read_cut();
+    } else {
+      gsync();   // (cluster: the bins are read; border's and make_list's barriers say so where there is a cut)
     }
   }
   if (by_p) {
