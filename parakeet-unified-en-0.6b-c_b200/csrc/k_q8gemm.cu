@@ -858,6 +858,11 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
+  // The commits' arrivals at the peer's barriers are no operations of the leader's
+  // threads, so the cluster's barrier does not order them before the peer's exit: the
+  // peer, too, waits for the last one.
+  if (rank == 1 && threadIdx.x == 32) mbar_wait(done, 0);
+  __syncwarp();
   // no CTA leaves (or frees its TMEM) while the pair's MMAs, loads or signals may reach it
   cluster_sync_all();
   if (warp == 1) {
