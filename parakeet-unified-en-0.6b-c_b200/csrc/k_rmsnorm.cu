@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int s
   extern __shared__ __align__(128) unsigned char ring_smem[];
   __shared__ unsigned long long full[G][RING_MAX];
   __shared__ float red[2][G][2][W];   // the row's partial sums and maxima; alternating
-  __shared__ int stop[G];
+  __shared__ int stop[2][G];          // a wait for this row ran out; alternating as well
   const int g = threadIdx.x / TPR, t = threadIdx.x % TPR, lane = t & 31, warp = t >> 5;
   const int nc = a.D / VEC;
   const unsigned row_bytes = (unsigned)a.D * sizeof(T), slot = a.y ? 2 * row_bytes : row_bytes;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int s
   if (t == 0) {
     for (int i = 0; i < stages; i++) mbar_init(&full[g][i], 1);
     mbar_init_fence();
-    stop[g] = 0;
+    stop[0][g] = stop[1][g] = 0;
     for (int i = 0; i < stages; i++)
       if (first + i * step < a.n_rows) load(first + i * step, i);
   }
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int s
     const bool here = mbar_wait(&full[g][at], phase);
     if (!here) {
       if (t == 0) atomicAdd(&g_wait_timeouts, 1u);
-      stop[g] = 1;
+      stop[flip][g] = 1;
     }
     const Pack<T, VEC> *sx = reinterpret_cast<const Pack<T, VEC> *>(ring + at * slot);
     const Pack<T, VEC> *sy = reinterpret_cast<const Pack<T, VEC> *>(ring + at * slot + row_bytes);
@@ -411,7 +411,9 @@ __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int s
       red[flip][g][1][warp] = amax;
     }
     asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(TPR) : "memory");
-    if (*(volatile int *)&stop[g]) break;
+    // the whole group reads this row's word and leaves together: a thread that is ahead,
+    // and whose wait for the next row runs out, writes the other one
+    if (*(volatile int *)&stop[flip][g]) break;
     if (t == 0 && row + stages * step < a.n_rows) load(row + stages * step, at);
     ss = red[flip][g][0][0];
     amax = red[flip][g][1][0];
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(TPR *G, 1) rms_q8_ring_kernel(RmsArgs a, int s
   }
   // a wait ran out: the copies still in flight land (bounded) before the CTA's
   // shared memory is released
-  if (t == 0 && *(volatile int *)&stop[g])
+  if (t == 0 && (*(volatile int *)&stop[0][g] | *(volatile int *)&stop[1][g]))
     for (int i = 0; i < stages; i++) {
       mbar_wait(&full[g][i], 0);
       mbar_wait(&full[g][i], 1);
