@@ -184,15 +184,22 @@ __device__ __forceinline__ void tmem_ld(unsigned taddr, unsigned (&r)[NC]) {
 
 // v / (1 + exp(-v)) on a pair: exp(-v) = 2^-h (1 + l ln 2) with h the rounded
 // product v log2 e and -l the rest of the exact one, 2^-h and the reciprocal by
-// the hardware's approximations (2 and 1 units in the last place). v counts as
-// -200 below that, and past 2^125 (v below -86) the power stands still: the
-// result is then within 5e-36 of 0.
+// the hardware's approximations (2 and 1 units in the last place). The power is
+// of v held to +-86, so that nothing in it overflows: above, 1 + exp(-v) is 1 and
+// the result v, infinity included; below, v counts as -86 in the product too, and
+// the result is within 5e-36 of 0. A NaN stays one.
+__device__ __forceinline__ float clamp_sym_nan(float v, float most) {   // min(|v|, most) with v's sign
+  float r;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  return r;
+}
 __device__ __forceinline__ float2 swish_ex2(float2 v) {
-  v = make_float2(max_nan(v.x, -200.0f), max_nan(v.y, -200.0f));
-  const float2 h = mul2(v, splat2(GATE_L2E_HI));
-  float2 l = fma2(v, splat2(-GATE_L2E_HI), h);
-  l = mul2(fma2(v, splat2(-GATE_L2E_LO), l), splat2(0.693147180559945f));
-  float2 e = make_float2(ex2_approx(fminf(-h.x, 125.0f)), ex2_approx(fminf(-h.y, 125.0f)));
+  const float2 t = make_float2(clamp_sym_nan(v.x, 86.0f), clamp_sym_nan(v.y, 86.0f));
+  v = make_float2(max_nan(v.x, -86.0f), max_nan(v.y, -86.0f));
+  const float2 h = mul2(t, splat2(GATE_L2E_HI));
+  float2 l = fma2(t, splat2(-GATE_L2E_HI), h);
+  l = mul2(fma2(t, splat2(-GATE_L2E_LO), l), splat2(0.693147180559945f));
+  float2 e = make_float2(ex2_approx(-h.x), ex2_approx(-h.y));
   e = fma2(e, l, e);
   const float2 d = add2(splat2(1.0f), e);
   return mul2(v, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
