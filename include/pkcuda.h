@@ -312,7 +312,8 @@ int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, f
  *                                    sum_k A[m, k] W[k, n] + bias[n])
  * int8 x int8 summed exactly in 32-bit integers, e4m3 x e4m3 in the tensor
  * cores' fp32 accumulators (within 2^-22 of the terms' magnitudes per 32 of K);
- * the rest in fp32, rounded once to C's type.
+ * the rest in fp32 (the GELU of v within (2 v^2 + 20) 2^-24 of its value, the
+ * Swish and tanh within 8 x 2^-24), rounded once to C's type.
  * A weight is prepared once (synchronous, on the current device): data [K, N]
  * row-major device memory of type I8 (-127 .. 127 in the reference's
  * checkpoints; -128 is taken as it is) or E4M3, scales fp32 device memory, 1

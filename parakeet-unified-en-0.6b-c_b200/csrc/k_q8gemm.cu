@@ -205,6 +205,34 @@ __device__ __forceinline__ float2 swish_ex2(float2 v) {
   return mul2(v, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
 }
 
+// v (1 + erf(v / sqrt 2)) / 2 on a pair, as max(v, 0) - g with g = |v| erfc(|v| / sqrt
+// 2) / 2: the form with erf leaves nothing of the values below v = -5 (1 + erf
+// cancels). g = a e^(-a^2 / 2) P(t), a = |v|, t = 1 / (1 + 0.3 a), where P is the
+// polynomial of degree 8 whose largest relative distance from erfcx(a / sqrt 2) / 2
+// over 0 <= a <= 13.5 is least (0.96 x 2^-24; by reweighted least squares). Within (2
+// v^2 + 20) 2^-24 of the value: a^2 / 2 is off by three roundings, the power by 4 x
+// 2^-24, t by 3, of which P shows 2.7 times as much at most, P's own steps 4, and the
+// products. a counts as 20 at most, where the power is 0: v stays, infinity
+// included, and -infinity gives 0. 12000 x 1024 x 4096 bf16 92 us with erff, 132 with
+// erfcf, 71 this way.
+__device__ __forceinline__ float2 gelu2(float2 v) {
+  const float2 a = make_float2(min_nan(fabsf(v.x), 20.0f), min_nan(fabsf(v.y), 20.0f));
+  const float2 d = fma2(a, splat2(0.3f), splat2(1.0f));
+  const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  const float2 s = mul2(mul2(a, a), splat2(-0.72134752044448170f));   // -log2(e) / 2
+  float2 p = splat2(0.038334265f);
+  p = fma2(p, t, splat2(-0.16895193f));
+  p = fma2(p, t, splat2(0.22821721f));
+  p = fma2(p, t, splat2(-0.075999506f));
+  p = fma2(p, t, splat2(0.142185f));
+  p = fma2(p, t, splat2(0.094833f));
+  p = fma2(p, t, splat2(0.12188206f));
+  p = fma2(p, t, splat2(0.11949307f));
+  p = fma2(p, t, splat2(6.8528907e-06f));
+  const float2 g = mul2(mul2(a, p), make_float2(ex2_approx(s.x), ex2_approx(s.y)));
+  return sub2(make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f)), g);
+}
+
 template <int NC>
 __device__ __forceinline__ void activate(int act, float (&v)[NC]) {
   switch (act) {
@@ -226,7 +254,11 @@ __device__ __forceinline__ void activate(int act, float (&v)[NC]) {
       break;
     case PKCU_ACT_GELU:
 #pragma unroll
-      for (int j = 0; j < NC; j++) v[j] = 0.5f * v[j] * (1.0f + erff(v[j] * 0.70710678118654752f));
+      for (int j = 0; j < NC; j += 2) {
+        const float2 s = gelu2(make_float2(v[j], v[j + 1]));
+        v[j] = s.x;
+        v[j + 1] = s.y;
+      }
       break;
     default: break;
   }

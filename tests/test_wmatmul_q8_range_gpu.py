@@ -73,3 +73,24 @@ def test_whole_range(cuda, M, act, out):
 def test_nan_stays(cuda, M, act):
     v = np.full(N, math.nan, np.float32)
     assert np.isnan(values(cuda, M, "f32", act, v)).all()
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M", [1, 200, 2500])
+def test_gelu(cuda, M, out):
+    """The GELU's small values left of 0 have the relative error of the others.
+    g = |v| e^(-v^2 / 2) P: the exponent s = a^2 (log2 e) / 2 has three roundings (a^2,
+    the constant, their product), v^2 / 2 x 3 x 2^-24 of the power, whose approximation
+    is off by 2^-22; t = 1 / (1 + 0.3 |v|) by 3 x 2^-24 (the sum, the reciprocal's unit
+    in the last place), which P multiplies by |t P' / P| <= 2.7; P by its distance, 1,
+    and its steps, 4; two products round: (1.5 v^2 + 4 + 8.1 + 5 + 2) 2^-24 < (2 v^2 +
+    20) 2^-24, and the difference max(v, 0) - g once more where it is not exact. Where
+    the power is below fp32's normal numbers (|v| > 13.2) the value is below 1e-36."""
+    from scipy.special import erfc
+    v = np.concatenate([arguments()[:54], np.linspace(-14, -2, 601), np.linspace(-2, 9, 300)]).astype(np.float32)
+    v = np.resize(v, N)
+    x = v.astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want = np.where(x < -30, 0.0, 0.5 * x * erfc(-x / math.sqrt(2)))
+    fin = np.where(np.isinf(want), 0, np.abs(want))
+    compare(values(cuda, M, out, "gelu", v), want, (2 * np.minimum(x * x, 1e4) + 20) * U * fin + 1e-36, out)
