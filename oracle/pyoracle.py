@@ -56,6 +56,13 @@ def build(quiet: bool = True) -> None:
         print(out.stdout)
 
 
+def ref_tree() -> bool:
+    """Whether the reference tree that oracle/Makefile builds _ref/ from is there."""
+    out = subprocess.run(["make", "-s", "--no-print-directory", "-C", HERE, "have-ref"], capture_output=True, text=True,
+                         check=True)
+    return out.stdout.strip() == "yes"
+
+
 def _fp(a: np.ndarray):
     assert a.dtype == np.float32 and a.flags.c_contiguous
     return a.ctypes.data_as(FP)
