@@ -588,7 +588,7 @@ static int launch_dwconv(const float *x, const float *w, const float *b, const f
 
 using namespace pk;
 
-PK_WAIT_TIMEOUTS_ACCESSOR(pk_conv_wait_timeouts)
+PK_WAIT_WORD(pk_conv_wait_word)
 
 extern "C" int pkcu_glu(const float *in, const float *bias, float *out, int C, int layout,
                         const pkcu_seq *seq, pkcu_stream_t stream) {

@@ -934,7 +934,7 @@ __global__ void fill_scales_kernel(const float *__restrict__ scales, int n_scale
   if (i < N) out[i] = scales[n_scales == 1 ? 0 : i];
 }
 
-PK_WAIT_TIMEOUTS_ACCESSOR(pk_q8_wait_timeouts_acc)
+PK_WAIT_WORD(pk_q8_wait_word)
 
 }  // namespace q8
 }  // namespace pk
@@ -1105,8 +1105,6 @@ Plan plan(int M, int N, int nkb, bool c_vec) {
   return best;
 }
 }  // namespace
-
-extern "C" int pk_q8_wait_timeouts(unsigned *count, int reset) { return q8::pk_q8_wait_timeouts_acc(count, reset); }
 
 extern "C" void pkcu_weight_q8_destroy(pkcu_weight_q8 *w) {
   if (!w) return;

@@ -512,7 +512,7 @@ int rms_launch(const RmsArgs &a, int e4m3, cudaStream_t s) {
 
 using namespace pk;
 
-PK_WAIT_TIMEOUTS_ACCESSOR(pk_rms_wait_timeouts)
+PK_WAIT_WORD(pk_rms_wait_word)
 
 extern "C" int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, float alpha,
                                          const float *gamma, float eps, int dtype, void *x_out, void *q,

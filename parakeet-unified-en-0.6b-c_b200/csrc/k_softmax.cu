@@ -635,7 +635,7 @@ static int check_scores(const float *ac, const float *bd, const float *S, const 
 
 using namespace pk;
 
-PK_WAIT_TIMEOUTS_ACCESSOR(pk_softmax_wait_timeouts)
+PK_WAIT_WORD(pk_softmax_wait_word)
 
 extern "C" int pkcu_softmax_rows(float *x, int n_rows, int len, pkcu_stream_t stream) {
   if (!x || n_rows < 0 || len <= 0) return pkcu_fail(PKCU_ERR_ARG, "pkcu_softmax_rows: bad argument");

@@ -765,7 +765,7 @@ __global__ void split_t_pad_kernel(const float *__restrict__ X, __nv_bfloat16 *_
   }
 }
 
-PK_WAIT_TIMEOUTS_ACCESSOR(pk_tc_wait_timeouts_acc)
+PK_WAIT_WORD(pk_tc_wait_word)
 
 }  // namespace tc
 }  // namespace pk
@@ -848,10 +848,6 @@ extern "C" void pk_tc_warm(void) {
   smem_optin(tc::tc_gemm_kernel<3, 64>, tc::Cfg<3, 64>::SMEM, optin_flags<3, 64>());
   smem_optin(tc::tc_gemm_kernel<1, 128>, tc::Cfg<1, 128>::SMEM, optin_flags<1, 128>());
   smem_optin(tc::tc_gemm_kernel<3, 128>, tc::Cfg<3, 128>::SMEM, optin_flags<3, 128>());
-}
-
-extern "C" int pk_tc_wait_timeouts(unsigned *count, int reset) {
-  return tc::pk_tc_wait_timeouts_acc(count, reset);
 }
 
 extern "C" int pk_tc_prepare(const void *data, int bits, float scale, int K, int N, void *planes,

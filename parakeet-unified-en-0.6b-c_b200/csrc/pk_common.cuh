@@ -455,19 +455,13 @@ constexpr unsigned long long PK_WAIT_NS = 1000000000ULL;   // 1 s per wait
 // Waits that ran out in this translation unit's kernels since the last reset.
 static __device__ unsigned g_wait_timeouts;
 
-// Host accessor of g_wait_timeouts for one translation unit (current device).
-#define PK_WAIT_TIMEOUTS_ACCESSOR(fn)                                              \
-  extern "C" int fn(unsigned *count, int reset) {                                  \
-    unsigned v = 0;                                                                \
-    if (cudaMemcpyFromSymbol(&v, pk::g_wait_timeouts, sizeof v) != cudaSuccess)    \
-      return PKCU_ERR_CUDA;                                                        \
-    if (reset) {                                                                   \
-      const unsigned zero = 0;                                                     \
-      if (cudaMemcpyToSymbol(pk::g_wait_timeouts, &zero, sizeof zero) != cudaSuccess) \
-        return PKCU_ERR_CUDA;                                                      \
-    }                                                                              \
-    *count = v;                                                                    \
-    return PKCU_OK;                                                                \
+// Its device address for one translation unit (current device), for pk_waits.cu.
+#define PK_WAIT_WORD(fn)                                                                     \
+  extern "C" int fn(unsigned **word) {                                                       \
+    return cudaGetSymbolAddress(reinterpret_cast<void **>(word), pk::g_wait_timeouts) ==     \
+                   cudaSuccess                                                               \
+               ? PKCU_OK                                                                     \
+               : PKCU_ERR_CUDA;                                                              \
   }
 
 // Waits until phase `parity` of bar has completed, at most `limit_ns`.

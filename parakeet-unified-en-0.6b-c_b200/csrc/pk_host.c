@@ -65,27 +65,20 @@ int pkcu_device(void)
 int pkcu_wait_timeouts(unsigned *count, int reset)
 {
     if (!count) return pkcu_fail(PKCU_ERR_ARG, "pkcu_wait_timeouts: NULL count");
-    unsigned a = 0, b = 0, c = 0, d = 0, e = 0;
-    if (pk_softmax_wait_timeouts(&a, reset) != PKCU_OK || pk_conv_wait_timeouts(&b, reset) != PKCU_OK ||
-        pk_tc_wait_timeouts(&c, reset) != PKCU_OK || pk_q8_wait_timeouts(&d, reset) != PKCU_OK ||
-        pk_rms_wait_timeouts(&e, reset) != PKCU_OK)
+    if (pk_wait_timeouts(count, reset) != PKCU_OK)
         return pkcu_fail(PKCU_ERR_CUDA, "pkcu_wait_timeouts: reading the device counters failed");
-    *count = a + b + c + d + e;
     return PKCU_OK;
 }
 
 int pk_check_wait_timeouts(const char *what)
 {
-    unsigned a = 0, b = 0, c = 0, d = 0, e = 0;
-    if (pk_softmax_wait_timeouts(&a, 1) != PKCU_OK || pk_conv_wait_timeouts(&b, 1) != PKCU_OK ||
-        pk_tc_wait_timeouts(&c, 1) != PKCU_OK || pk_q8_wait_timeouts(&d, 1) != PKCU_OK ||
-        pk_rms_wait_timeouts(&e, 1) != PKCU_OK) {
+    unsigned n = 0;
+    if (pk_wait_timeouts(&n, 1) != PKCU_OK) {
         cudaGetLastError();
         return pkcu_fail(PKCU_ERR_CUDA, "%s: reading the device wait counters failed", what);
     }
-    if (a + b + c + d + e)
-        return pkcu_fail(PKCU_ERR_CUDA, "%s: %u bounded device wait(s) ran out; outputs are incomplete",
-                         what, a + b + c + d + e);
+    if (n)
+        return pkcu_fail(PKCU_ERR_CUDA, "%s: %u bounded device wait(s) ran out; outputs are incomplete", what, n);
     return PKCU_OK;
 }
 

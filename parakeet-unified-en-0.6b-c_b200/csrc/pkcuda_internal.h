@@ -48,14 +48,16 @@ int pkcu_launch_status(const char *what);
 int pkcu_sm_count(void);
 /* Current device index, or 0. */
 int pkcu_device(void);
-/* Per-translation-unit counters of device waits that ran out (k_softmax.cu,
- * k_conv.cu); read and optionally reset on the current device. */
-int pk_softmax_wait_timeouts(unsigned *count, int reset);
-int pk_conv_wait_timeouts(unsigned *count, int reset);
-int pk_tc_wait_timeouts(unsigned *count, int reset);   /* k_tcgemm.cu */
+/* Device waits that ran out on the current device, of all translation units
+ * together; read and optionally reset (pk_waits.cu). */
+int pk_wait_timeouts(unsigned *count, int reset);
+/* The device word in which each unit counts them. */
+int pk_softmax_wait_word(unsigned **word);
+int pk_conv_wait_word(unsigned **word);
+int pk_tc_wait_word(unsigned **word);
+int pk_q8_wait_word(unsigned **word);
+int pk_rms_wait_word(unsigned **word);
 
-int pk_q8_wait_timeouts(unsigned *count, int reset);   /* k_q8gemm.cu */
-int pk_rms_wait_timeouts(unsigned *count, int reset);  /* k_rmsnorm.cu */
 /* The driver's cuTensorMapEncodeTiled (looked up once, k_tcgemm.cu). */
 int pk_tensor_map_encoder(void **fn);
 
@@ -112,7 +114,7 @@ int pk_split_rows_cat(const float *X1, const float *X2, void *parts, long long M
 int pk_split_cf_t(const float *X, void *parts, int C, const pkcu_seq *seq, pkcu_stream_t stream);
 
 /* For synchronous entry points, after their final synchronisation: reads and
- * resets both counters and returns PKCU_ERR_CUDA (with a message naming what)
+ * resets the counters and returns PKCU_ERR_CUDA (with a message naming what)
  * when any wait ran out since the last reset, anywhere in the process on this
  * device. */
 int pk_check_wait_timeouts(const char *what);
