@@ -305,6 +305,13 @@ def _require(ok, what) -> None:
         raise ValueError(what)
 
 
+def _ints32(what, *sizes):
+    """Sizes go to C as int, which ctypes would cut to 32 bits without a word."""
+    for n in sizes:
+        if n > 0x7fffffff:
+            raise ValueError(f"{what}: {n} is more than a 32-bit size")
+
+
 def _vector(t, n, dev, what):
     """Address of a packed fp32 tensor of n entries on device dev (None for None)."""
     if t is None:
@@ -345,6 +352,8 @@ def residual_rms_norm_q8(x, y, bias, alpha, gamma, eps, x_out, q, scales, stream
     if len(shape) != 2 or dev < 0 or not x.is_contiguous():
         raise ValueError("x: a packed [n_rows, D] CUDA tensor is needed")
     rows, D = shape
+    if (rows | D) >> 31:
+        _ints32("x", rows, D)
     for t in (y, x_out):
         if t is not None and t is not x and not (
                 t.dtype is x.dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
@@ -367,6 +376,7 @@ class WeightQ8:
         self.handle = VP()
         _require(data.dim() == 2 and data.is_cuda and data.is_contiguous(), "data: a packed [K, N] CUDA tensor is needed")
         K, N = data.shape
+        _ints32("data", K, N)
         if not torch.is_tensor(scales):
             with torch.cuda.stream(stream):   # None: the current one
                 scales = torch.full((1,), float(scales), device=data.device)
@@ -415,6 +425,8 @@ def wmatmul_q8(a, a_scales, weight, out, bias=None, act=None, residual=None, rsc
     if step != 1 or dev < 0 or a.dtype is not weight.dtype or ashape[1] < weight.K:
         raise ValueError("a: [M, >= K] of the weight's type with packed columns is needed")
     M = ashape[0]
+    if M >> 31:
+        _ints32("a", M)
     ldc, ldr, r = 0, 0, None
     for t in (out, residual):
         if t is None:
@@ -443,6 +455,8 @@ def sample_rows(logits, u, tokens, logprobs=None, temperature=None, top_k=None, 
     if len(shape) != 2 or dev < 0 or (step != 1 and shape[1] > 1):
         raise ValueError("logits: [n_rows, V] on the GPU with packed columns is needed")
     rows, V = shape
+    if V >> 31:
+        _ints32("logits", V)
     _on(dev, stream, "pkcu_sample_rows", logits.data_ptr(), dtype, ld if rows > 1 else max(ld, V),
         _vector(temperature, rows, dev, "temperature"), _ints(top_k, rows, dev, "top_k"),
         _vector(top_p, rows, dev, "top_p"), _vector(min_p, rows, dev, "min_p"), _vector(u, rows, dev, "u"),
