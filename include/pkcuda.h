@@ -295,12 +295,13 @@ int pkcu_argmax_rows(const float *logits, int32_t *out, long long n_rows, int V,
  *   q      = n / scales rounded to nearest even, [n_rows, ldq] bytes (columns
  *            from D on are left as they were)
  * Arithmetic in fp32. x_out may be x. y NULL: no residual (bias must be NULL
- * too), the norm is of x, and x_out may be NULL. bias may be NULL. A row of
- * zeros gives q = 0 and scale 0; a row with a NaN or an infinity, or whose sum
- * of squares passes fp32's range (1024 entries of 6e17), q = 0 and scale NaN. ldq a multiple of 16
- * and q 16-byte aligned make the rows an operand of pkcu_wmatmul_q8. Pointers
- * aligned to their type; 16-byte alignment (and D a multiple of 4, of 8 in 16
- * bits) is the fast case. */
+ * too), the norm is of x, and x_out may be NULL. bias may be NULL. D 1 .. 2^24,
+ * eps positive and finite. A row of zeros gives q = 0 and scale 0. q = 0 and
+ * scale NaN: a row with a NaN or an infinity, and one past fp32's range in its
+ * sum of squares (1024 entries of 6e17) or in an x_out * gamma. ldq a multiple
+ * of 16 and q 16-byte aligned make the rows an operand of pkcu_wmatmul_q8.
+ * Pointers aligned to their type; 16-byte alignment (and D a multiple of 4, of
+ * 8 in 16 bits) is the fast case. */
 int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, float alpha,
                               const float *gamma, float eps, int dtype, void *x_out, void *q,
                               int qtype, long long ldq, float *scales, int n_rows, int D,

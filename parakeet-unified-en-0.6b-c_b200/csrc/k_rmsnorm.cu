@@ -57,13 +57,17 @@ __device__ __forceinline__ bool row_finite(float ss, float amax) { return ss < I
 constexpr float kTiny = 0x1p-100f, kTinyUp = 0x1p100f;
 
 // The row's scale (one thread): a NaN or an infinity anywhere in the row (or
-// squares past fp32) makes it NaN, so that every entry stands for NaN.
+// squares or an x' gamma past fp32) makes it NaN, so that every entry stands for
+// NaN. Not kept: such finite rows once more from memory, with scaled squares and
+// products; the path, never taken, cost 1 to 4 % of every row's time (2049 x 8192 bf16
+// to e4m3 31.5 us and 32.7, 12000 x 300 fp32 11.2 and 11.6), called, inlined or behind
+// the ring's loop.
 template <bool E4M3>
 __device__ __forceinline__ float row_scale(float ss, float amax, float eps, int D) {
   if (!row_finite(ss, amax)) return __int_as_float(0x7fffffff);
   if (amax == 0.0f) return 0.0f;
-  const float r = 1.0f / sqrtf(ss / (float)D + eps);
-  return amax * r / Quant<E4M3>::Q;
+  const float r = 1.0f / sqrtf(ss / (float)D + eps), top = amax * r;   // top: of the norm, perhaps past fp32
+  return top < INFINITY ? top / Quant<E4M3>::Q : amax * (r / Quant<E4M3>::Q);
 }
 // Q / max|t| (max|t| times up, what t is multiplied by first), 0 for a row whose q
 // is 0; lo (e4m3): what its rounding left.
