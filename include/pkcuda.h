@@ -319,14 +319,15 @@ int pkcu_residual_rms_norm_q8(const void *x, const void *y, const float *bias, f
  * row-major device memory of type I8 (-127 .. 127 in the reference's
  * checkpoints; -128 is taken as it is) or E4M3, scales fp32 device memory, 1
  * for the whole weight (the reference's int8 storage) or N, one per column.
- * K up to 131071; no divisibility is asked of K or N. */
+ * K up to 131071, N (and M below) up to 2147483392; no divisibility is asked
+ * of K or N. */
 typedef struct pkcu_weight_q8 pkcu_weight_q8;
 int  pkcu_weight_q8_create(const void *data, int dtype, const float *scales, int n_scales, int K,
                            int N, pkcu_stream_t stream, pkcu_weight_q8 **out);
 void pkcu_weight_q8_destroy(pkcu_weight_q8 *w);
 /* A [M, lda] bytes of the weight's type, K of each row used (lda a multiple of
- * 16, A 16-byte aligned: pkcu_residual_rms_norm_q8 writes such rows), a_scales
- * [M]; bias [N] or NULL; act PKCU_ACT_*; R [M, ldr] or NULL (nothing added) and
+ * 16 below 2^40, A 16-byte aligned: pkcu_residual_rms_norm_q8 writes such rows),
+ * a_scales [M]; bias [N] or NULL; act PKCU_ACT_*; R [M, ldr] or NULL (nothing added) and
  * C [M, ldc] of type dtype (F32, BF16 or F16), pitches in entries; R may be C.
  * No work buffer; calls of one weight may run at the same time. */
 int  pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scales, const pkcu_weight_q8 *W,

@@ -35,8 +35,6 @@
 #include <stdlib.h>
 #include <string.h>
 
-#include <mutex>
-
 #include "pk_common.cuh"
 #include "pk_types.cuh"
 
@@ -609,8 +607,15 @@ __device__ __forceinline__ void umma_commit_pair(unsigned long long *bar) {
       "h"((unsigned short)3)
       : "memory");
 }
-// Relaxed: what it announces is that TMEM reads are done (waited for before).
-// A release would also wait for the stores to C in flight, 3000 cycles a tile.
+// Relaxed: what it announces is that TMEM reads are done, and no memory operation.
+// tcgen05.wait::ld has completed them (their registers are written), and
+// tcgen05.fence::before_thread_sync ahead of the arrival with
+// tcgen05.fence::after_thread_sync behind the waiter's observing it order tcgen05
+// operations across threads whatever the semantics of the arrival itself (PTX's
+// memory consistency model for tcgen05: the fences make an execution ordering
+// instruction, a relaxed mbarrier operation among them, order what stands before
+// the one before what stands behind the other). A release would also wait for the
+// stores to C in flight, 3000 cycles a tile.
 __device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -914,7 +919,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // ── weight preparation (once per weight) ─────────────────────────────────────
 
 // W [K, N] bytes -> [N, Kp] bytes, zeros from column K on: 64 x 64 tiles through
-// shared memory, reads along N and writes along K in 4-byte words.
+// shared memory, reads along N and writes along K, byte by byte.
 __global__ void prep_q8_kernel(const unsigned char *__restrict__ W, unsigned char *__restrict__ out, int K, int N,
                                int Kp) {
   __shared__ unsigned char tile[64][65];
