@@ -21,8 +21,9 @@
 // kernel's launch alone are 3 us of the first two).
 //
 // Many tokens (q8_pair_kernel): 256 x 256 tiles of CTA pairs. 12000 x 1024 x 4096
-// int8 to bf16 51 us, with Swish 62 to 66; 12000 x 4096 x 1024 with an fp32 residual
-// 55 us; 8192^3 375 us = 2.9 Pop/s, 0.90 of twice the measured bf16 GEMM rate.
+// int8 to bf16 50 us, with Swish 63 to 66, with GELU 71; 12000 x 4096 x 1024 with an
+// fp32 residual 55 us; 8192^3 375 to 395 us = 2.8 to 2.9 Pop/s, 0.85 to 0.90 of twice the
+// measured bf16 GEMM rate.
 //
 // Operands. Rows of 128 bytes of K per stage, 128-byte swizzled, by TMA (no
 // multicast); K needs no alignment: the tensor maps' extent is K itself, so

@@ -14,11 +14,12 @@
 // bytes of HBM traffic per element in fp32, 7 in 16 bits. That traffic is the
 // bound in fp32: 12000 x 1024 to int8 in 28.0 us = 5.7 TB/s, 0.87 of the copy
 // bandwidth, to e4m3 28.7; 4000 x 4096 0.88. 16-bit rows take 0.8 of the time for 0.54
-// of the bytes (12000 x 1024 bf16 22.4 us = 0.59): 35 instructions per entry, of which
-// the row's own part (addresses, reduction, scale) is half, and gamma's and bias's fp32
-// reads through L1 weigh twice as much. Wide 16-bit rows where they are many come
-// through shared memory by bulk copies (2049 x 8192 to int8 0.70 without a bias, 6000 x
-// 8192 0.80; 1024-wide rows 24 to 28 us that way). Measured and not kept: persistent
+// of the bytes (12000 x 1024 bf16 22.4 us = 0.59): issue slots are 62 % busy with 35
+// instructions per entry, and the warps wait for loads (10.5 of them on the long
+// scoreboard per issue), of which gamma's and bias's, fp32 through L1 again for every
+// row, are twice the bytes of the row's own. Wide 16-bit rows where they are many come
+// through shared memory by bulk copies (2049 x 8192 to int8 without a bias 24.6 us = 0.73,
+// 6000 x 8192 0.89; 1024-wide rows 24 to 28 us that way). Measured and not kept: persistent
 // CTAs that load the next row into registers before they finish this one (34 to 44 us
 // fp32, 25 to 33 bf16), rows kept packed in 16 bits between the two looks at them.
 #include <cuda_bf16.h>
