@@ -350,7 +350,8 @@ int  pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scales, const 
  * token's weight over that total. Logits of -infinity and NaN are never taken;
  * a row with nothing else gives token -1 and log-probability -infinity. Weights
  * are held to 2^-44 of the largest and summed exactly: the result does not
- * depend on the order of any sum, and what weighs less is never drawn. */
+ * depend on the order of any sum, what weighs less is never drawn, and a
+ * log-probability is off by at most 2^-45 per kept entry and its rounding. */
 int pkcu_sample_rows(const void *logits, int dtype, long long ld, const float *temperature,
                      const int32_t *top_k, const float *top_p, const float *min_p,
                      const float *u, int32_t *tokens, float *logprobs, long long n_rows, int V,

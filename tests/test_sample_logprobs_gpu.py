@@ -1,8 +1,9 @@
 """GPU: pkcu_sample_rows' log-probabilities are the definition's, rounded once.
 
 In fp64 the exponent is off by 4 x 2^-53 of its value (at most 60 here) and the
-logarithm by as much as the sum, 2^18 weights of 2 x 10^-13 and 2^-45 each: below
-10^-11 in all; the result rounds to fp32 by 2^-24 of its value."""
+logarithm by 4 x 10^-13 and as much as the sum: 2 x 10^-13 of it, and 2^-45 of the
+largest weight per entry at most, for these rows 2.1 x 10^-12 together (computed from
+them); the result rounds to fp32 by 2^-24 of its value."""
 import numpy as np
 import pytest
 
