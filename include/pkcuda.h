@@ -327,8 +327,9 @@ int  pkcu_weight_q8_create(const void *data, int dtype, const float *scales, int
 void pkcu_weight_q8_destroy(pkcu_weight_q8 *w);
 /* A [M, lda] bytes of the weight's type, K of each row used (lda a multiple of
  * 16 below 2^40, A 16-byte aligned: pkcu_residual_rms_norm_q8 writes such rows),
- * a_scales [M]; bias [N] or NULL; act PKCU_ACT_*; R [M, ldr] or NULL (nothing added) and
- * C [M, ldc] of type dtype (F32, BF16 or F16), pitches in entries; R may be C.
+ * a_scales [M]; bias [N] or NULL; act PKCU_ACT_*; R [M, ldr] or NULL (nothing
+ * added) and C [M, ldc] of type dtype (F32, BF16 or F16), pitches in entries; R
+ * may be C.
  * No work buffer; calls of one weight may run at the same time. */
 int  pkcu_wmatmul_q8(const void *A, long long lda, const float *a_scales, const pkcu_weight_q8 *W,
                      const float *bias, int act, const void *R, long long ldr, float rscale,

@@ -35,9 +35,13 @@ extern "C" int pk_wait_timeouts(unsigned *count, int reset) {
   if (pk_softmax_wait_word(&w.at[0]) || pk_conv_wait_word(&w.at[1]) || pk_tc_wait_word(&w.at[2]) ||
       pk_q8_wait_word(&w.at[3]) || pk_rms_wait_word(&w.at[4]))
     return PKCU_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(32);
   std::lock_guard<std::mutex> lock(g_sum_lock);
-  sum_waits_kernel<<<1, 32>>>(w, reset);
-  if (cudaGetLastError() != cudaSuccess || cudaMemcpyFromSymbol(count, g_sum, sizeof *count) != cudaSuccess)
+  // (the launch's own status: an error that another call left behind is not this one's)
+  if (cudaLaunchKernelEx(&cfg, sum_waits_kernel, w, reset) != cudaSuccess ||
+      cudaMemcpyFromSymbol(count, g_sum, sizeof *count) != cudaSuccess)
     return PKCU_ERR_CUDA;
   return PKCU_OK;
 }

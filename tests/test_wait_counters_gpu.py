@@ -53,3 +53,27 @@ def test_a_synchronous_call_reports_and_clears(cuda, unit):
     L.pk_layer_norm_rows(p(x), p(g), p(b), p(o), 2, 1024)
     assert "3 bounded device wait(s) ran out" in L.pkcu_last_error().decode()
     assert read(cuda, 0) == 0
+
+
+def test_two_threads(cuda):
+    """Calls from several host threads at once: no count is lost or told twice."""
+    import threading
+    import torch
+    ws = words(cuda)
+    for i, w in enumerate(ws):
+        w.fill_(1 << i)
+    torch.cuda.synchronize()
+    seen, lock = [], threading.Lock()
+
+    def run():
+        torch.cuda.set_device(0)
+        for _ in range(50):
+            n = read(cuda, 1)
+            with lock:
+                seen.append(n)
+    threads = [threading.Thread(target=run) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(seen)[-1] == 31 and sum(seen) == 31
